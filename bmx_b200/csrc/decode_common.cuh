@@ -53,6 +53,38 @@ struct TileCursor {
   }
 };
 
+// Which pages of a sequence a kernel walks and which of their tokens a query sees (template parameter WALK of the kernels).
+//   WALK_ALL      every committed page
+//   WALK_OWN      the pages behind the first skip[b] ones (those are a prefix shared with other sequences, attended once for all of them)
+//   WALK_SLIDING  the newest token's window (the last `window` positions, its own among them) and the first `sinks` tokens of the
+//                 sequence; the pages between them are not touched, their page-table entries may be anything
+constexpr int WALK_ALL = 0, WALK_OWN = 1, WALK_SLIDING = 2;
+struct K2bWalk {
+  const int32_t* skip;
+  const int32_t* tail_len;  // WALK_SLIDING: tokens in the fp16 window, or null
+  int tail_cap;
+  int64_t window;
+  int64_t sinks;
+};
+// Tile j of a sequence is page j for j < keep and page j + gap behind; token t is visible iff t < sinks or t >= first.
+struct PageSpan {
+  int tiles, keep, gap;
+  int64_t first;
+};
+template <int WALK>
+__device__ __forceinline__ PageSpan page_span(const K2bWalk& w, int n_pages, int b) {
+  PageSpan s = {n_pages, 0, 0, 0};
+  if constexpr (WALK == WALK_OWN) s.gap = min(max(w.skip[b], 0), n_pages);
+  if constexpr (WALK == WALK_SLIDING) {
+    const int64_t total = (int64_t)n_pages * TILE_TOKENS + (w.tail_len ? min(w.tail_len[b], w.tail_cap) : 0);
+    s.first = max((int64_t)0, total - w.window);
+    s.keep = (int)min((int64_t)n_pages, (w.sinks + TILE_TOKENS - 1) / TILE_TOKENS);
+    s.gap = max(0, (int)min((int64_t)n_pages, s.first / TILE_TOKENS) - s.keep);
+  }
+  s.tiles = n_pages - s.gap;
+  return s;
+}
+
 struct K2bMergeParams {
   K2bGeom g;
   const __half* q;
@@ -70,7 +102,11 @@ struct K2bMergeParams {
   int out_dtype;
   float* partial_out;
   int n_sub;  // partial records per (CTA, sequence, head): record of sub s sits s*(main_grid + batch*h_kv) slots further
+  K2bWalk walk;
+  const float* prefix_part;  // WALK_OWN: records of the shared prefix, prefix_split per (sequence, query head)
+  int prefix_split;
 };
+constexpr int PREFIX_PART_STRIDE = 132;  // floats per record of a shared prefix: 128 accumulators, max (log2 units), sum, 2 unused
 
 struct K2bDecodeParams {
   K2bGeom g;
@@ -91,6 +127,7 @@ struct K2bDecodeParams {
   float* part;       // (grid + batch*h_kv, n_q_groups, PART_STRIDE)
   int32_t* status;
   int n_stages;
+  K2bWalk walk;
 };
 
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000LL;  // ~2 s at 2 GHz
@@ -141,8 +178,8 @@ int num_sms();
 // `after_main`: the page-streaming kernel of the same step was launched just before on the same stream.  The merge
 // kernel is then launched as its programmatic dependent: its blocks may start while that kernel drains, attend over
 // the fp16 window (which that kernel does not write) and wait for it only before they read the partial states.
-int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = false);
+int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = false, int walk = WALK_ALL);
 // tcgen05 decode kernel for layout-1 pools (k2b_decode_t5.cu); two partial records per slot (one per tile parity)
-int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s);
+int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk = WALK_ALL);
 
 }  // namespace bmxk

@@ -26,7 +26,7 @@
 #include <cstring>
 #include <mutex>
 
-#include "decode_common.cuh"
+#include "prefill_common.cuh"
 
 namespace bmxk {
 
@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) k2b_decode_kernel(const K2bDec
 // ---------------------------------------------------------------------------------------------
 constexpr int MERGE_THREADS = 256;
 
+template <int WALK>
 __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMergeParams p) {
   extern __shared__ __align__(16) float msm[];
   const K2bGeom g = p.g;
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   if (warp == 0) {
     int pre = 0, tot = 0;
     for (int i = lane; i < p.batch; i += 32) {
-      const int t = tiles_of(p.n_pages[i], g.page) * g.h_kv;
+      const int t = (WALK == WALK_ALL ? tiles_of(p.n_pages[i], g.page) : page_span<WALK>(p.walk, p.n_pages[i], i).tiles) * g.h_kv;
       tot += t;
       if (i < b) pre += t;
     }
@@ -452,6 +453,14 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   const int tl = p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
   const __half* kt = p.k_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
   const __half* vt = p.v_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
+  // WALK_SLIDING: window tokens [hid0, hid1) lie behind the sinks and in front of the sliding window: left out
+  int hid0 = 0, hid1 = 0;
+  if constexpr (WALK == WALK_SLIDING) {
+    const int64_t tail0 = (int64_t)p.n_pages[b] * TILE_TOKENS;
+    hid0 = (int)max((int64_t)0, min((int64_t)tl, p.walk.sinks - tail0));
+    hid1 = max(hid0, (int)max((int64_t)0, tl - p.walk.window));
+  }
+  auto shown = [&](int t) { return t < tl && (WALK != WALK_SLIDING || t < hid0 || t >= hid1); };
   float mx = -INFINITY;
   {
     const int l8 = tid & 7, tp = tid >> 3;
@@ -479,9 +488,11 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
         d += __shfl_xor_sync(0xffffffffu, d, 1);
         d += __shfl_xor_sync(0xffffffffu, d, 2);
         d += __shfl_xor_sync(0xffffffffu, d, 4);
-        if (t < tl) {
+        if (shown(t)) {
           mx = fmaxf(mx, d);
           if (l8 == 0) sc[t] = d;
+        } else if (WALK == WALK_SLIDING && t < tl && l8 == 0) {
+          sc[t] = -INFINITY;
         }
       }
     }
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int t = tg + 16 * i;
-    vv[i] = (t < tl) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
+    vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
@@ -523,7 +534,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = t0 + tg + 16 * i;
-          vv[i] = (t < tl) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
+          vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
         }
       }
 #pragma unroll
@@ -558,7 +569,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   //      CTA cta0 + r % n_cta.  Thread = (record parity, channel): an online softmax over its records ----
   const int total = si[1];
   const int per_cta = max(1, (total + p.main_grid - 1) / p.main_grid);
-  const int tiles_b = tiles_of(p.n_pages[b], g.page);
+  const int tiles_b = (WALK == WALK_ALL) ? tiles_of(p.n_pages[b], g.page) : page_span<WALK>(p.walk, p.n_pages[b], b).tiles;
   const int T0 = si[0] + h * tiles_b, T1 = T0 + tiles_b;
   const int cta0 = T0 / per_cta, cta1 = (tiles_b > 0) ? (T1 - 1) / per_cta : cta0 - 1;
   const int sub_slots = p.main_grid + p.batch * g.h_kv;
@@ -590,6 +601,28 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
         L = L * fo + l_[j] * fn, A = A * fo + a_[j] * fn, M = Mn;
       }
     }
+    if constexpr (WALK == WALK_OWN) {
+      // the shared prefix's records of this row (same units: the value rotation is undone below, once for both)
+      const float* pr = p.prefix_part + ((int64_t)bh * G + qi) * p.prefix_split * PREFIX_PART_STRIDE;
+      const int n_pre = p.walk.skip[b] > 0 ? p.prefix_split : 0;
+      for (int r0 = half; r0 < n_pre; r0 += 8) {
+        float m_[4], l_[4], a_[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = r0 + 2 * j;
+          const float* ps = pr + (int64_t)r * PREFIX_PART_STRIDE;
+          if (r < n_pre) m_[j] = ps[128], l_[j] = ps[129], a_[j] = ps[ch];
+          else m_[j] = -INFINITY, l_[j] = 0.f, a_[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float Mn = fmaxf(M, m_[j]);
+          const float fo = (M == -INFINITY) ? 0.f : ex2_approx(M - Mn);
+          const float fn = (m_[j] == -INFINITY) ? 0.f : ex2_approx(m_[j] - Mn);
+          L = L * fo + l_[j] * fn, A = A * fo + a_[j] * fn, M = Mn;
+        }
+      }
+    }
     red[half * HEAD_DIM + ch] = A;
     if (ch == 0) sm[16 + 2 * half] = M, sm[17 + 2 * half] = L;
   }
@@ -607,10 +640,12 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = x[k] * p.signs[4 * lane + k] * 0.08838834764831845f;
     }
+    // Nothing to attend to (an empty sequence): 0 in the walks that came with shared prefixes and sliding windows
     const float mw = (tl > 0) ? m_w : -INFINITY;
     const float Mf = fmaxf(Mp, mw);
     const float fp = (Mp == -INFINITY) ? 0.f : ex2_approx(Mp - Mf), fw = (mw == -INFINITY) ? 0.f : ex2_approx(mw - Mf);
-    const float l = Lp * fp + ((tl > 0) ? l_w : 0.f) * fw;
+    float l = Lp * fp + ((tl > 0) ? l_w : 0.f) * fw;
+    if (WALK != WALK_ALL && l == 0.f) l = 1.f;
     const int64_t row = (int64_t)bh * G + qi;
     float val[4];
 #pragma unroll
@@ -674,7 +709,7 @@ int num_sms() {
   return n;
 }
 
-int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main) {
+int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
   const int G = mp.g.n_q_groups;
   const size_t msmem = ((size_t)((mp.tail_cap + 3) & ~3) + (1 + 16 + 1) * HEAD_DIM + 32 + 4) * sizeof(float);
   BMXK_REQUIRE(msmem <= 48 * 1024, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
@@ -684,7 +719,9 @@ int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = after_main ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k2b_merge_kernel, mp);
+  const cudaError_t e = walk == WALK_OWN       ? cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_OWN>, mp)
+                        : walk == WALK_SLIDING ? cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_SLIDING>, mp)
+                                               : cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_ALL>, mp);
   if (e != cudaSuccess) {
     set_error("decode(merge): %s", cudaGetErrorString(e));
     return BMXK_ERR_CUDA;
@@ -734,12 +771,13 @@ size_t bmxk_k2b_decode_workspace_bytes(const bmxk_k2b_geom* g, int batch, int ma
   return 256 + slots * g->n_q_groups * PART_STRIDE * sizeof(float);
 }
 
-int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
-                    const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages,
-                    const void* rope_cos, const void* rope_sin, int64_t pos_offset, const void* k_tail,
-                    const void* v_tail, const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs,
-                    float sm_scale, void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* partial_out,
-                    int phases, void* stream) {
+}  // extern "C"
+
+// The checks of every decode entry point over a k2b pool; nothing is launched before they pass.
+static int check_step(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16, const int32_t* page_table,
+                      const int32_t* n_pages, int batch, int max_pages, const void* rope_cos, const void* rope_sin, const void* k_tail,
+                      const void* v_tail, const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, const void* workspace,
+                      size_t workspace_bytes, const void* out, int out_dtype, const float* partial_out, int phases) {
   BMXK_REQUIRE(g != nullptr, "bmxk_k2b_decode: null geometry");
   BMXK_REQUIRE(phases >= 1 && phases <= 3, "bmxk_k2b_decode: phases=%d must be 1, 2 or 3", phases);
   BMXK_REQUIRE(g->h_kv >= 1 && g->n_q_groups >= 1 && g->n_q_groups <= 8, "bmxk_k2b_decode: h_kv=%d n_q_groups=%d", g->h_kv,
@@ -763,19 +801,34 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
   BMXK_REQUIRE(out_dtype == BMXK_DTYPE_F16 || out_dtype == BMXK_DTYPE_F32, "bmxk_k2b_decode: out_dtype=%d", out_dtype);
   BMXK_REQUIRE(workspace_bytes >= bmxk_k2b_decode_workspace_bytes(g, batch, max_pages), "bmxk_k2b_decode: workspace too small");
   BMXK_REQUIRE(((uintptr_t)pages & 15) == 0 && ((uintptr_t)coefs & 15) == 0, "bmxk_k2b_decode: pools must be 16-byte aligned");
+  return BMXK_OK;
+}
+
+// One decode step over the pages that `walk` names (at most walk_pages of a sequence), the window and, for WALK_OWN, the records of the
+// shared prefixes; the entry points below check what is theirs.
+static int decode_step(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                    const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages,
+                    const void* rope_cos, const void* rope_sin, int64_t pos_offset, const void* k_tail,
+                    const void* v_tail, const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs,
+                    float sm_scale, void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* partial_out,
+                    int phases, int walk, const K2bWalk& w, int walk_pages, const float* prefix_part, int prefix_split, void* stream) {
+  const int bad = check_step(g, q, pages, coefs, basis_f16, page_table, n_pages, batch, max_pages, rope_cos, rope_sin, k_tail, v_tail, tail_len,
+                             tail_cap, v_lut, signs, workspace, workspace_bytes, out, out_dtype, partial_out, phases);
+  if (bad) return bad;
   cudaStream_t s = (cudaStream_t)stream;
 
   int32_t* status = reinterpret_cast<int32_t*>(workspace);
   float* part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + 256);
-  const int64_t max_tiles = (int64_t)batch * g->h_kv * (((int64_t)max_pages * g->page + TILE_TOKENS - 1) / TILE_TOKENS);
+  const int64_t max_tiles = (int64_t)batch * g->h_kv * (((int64_t)walk_pages * g->page + TILE_TOKENS - 1) / TILE_TOKENS);
   const int grid = (int)(max_tiles < num_sms() ? (max_tiles < 1 ? 1 : max_tiles) : num_sms());
   const float scale_log2 = sm_scale * 1.4426950408889634f;
   float alpha, beta;
   memcpy(&alpha, &v_lut[2], 4);
   memcpy(&beta, &v_lut[3], 4);
 
-  if (max_pages > 0 && (phases & 1)) {
+  if (walk_pages > 0 && (phases & 1)) {
     K2bDecodeParams prm;
+    prm.walk = w;
     prm.g.h_kv = g->h_kv, prm.g.n_q_groups = g->n_q_groups, prm.g.page = g->page, prm.g.rank = g->rank;
     prm.g.group = g->group, prm.g.n_coef_heads = g->n_coef_heads, prm.g.kbits = g->kbits, prm.g.vbits = g->vbits;
     prm.g.layout = g->layout;
@@ -786,7 +839,7 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
     prm.scale_log2 = scale_log2, prm.part = part, prm.status = status;
     if (g->layout == 1) {
       prm.n_stages = 0;
-      const int rc5 = launch_decode_t5(prm, grid, s);
+      const int rc5 = launch_decode_t5(prm, grid, s, walk);
       if (rc5) return rc5;
     } else {
     const size_t stage = decode_stage_bytes(g), fixed = decode_fixed_smem(batch);
@@ -812,7 +865,96 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
   mp.k_tail = (const __half*)k_tail, mp.v_tail = (const __half*)v_tail, mp.tail_len = tail_cap > 0 ? tail_len : nullptr;
   mp.tail_cap = tail_cap, mp.signs = signs, mp.scale_log2 = scale_log2, mp.out = out, mp.out_dtype = out_dtype;
   mp.partial_out = partial_out;
-  return launch_merge(mp, s, max_pages > 0 && (phases & 1));
+  mp.walk = w, mp.prefix_part = prefix_part, mp.prefix_split = prefix_split;
+  return launch_merge(mp, s, walk_pages > 0 && (phases & 1), walk);
+}
+
+extern "C" {
+
+int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                    const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages,
+                    const void* rope_cos, const void* rope_sin, int64_t pos_offset, const void* k_tail,
+                    const void* v_tail, const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs,
+                    float sm_scale, void* workspace, size_t workspace_bytes, void* out, int out_dtype, float* partial_out,
+                    int phases, void* stream) {
+  return decode_step(g, q, pages, coefs, basis_f16, page_table, table_stride, n_pages, batch, max_pages, rope_cos, rope_sin, pos_offset, k_tail,
+                     v_tail, tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, partial_out, phases, WALK_ALL,
+                     K2bWalk{}, max_pages, nullptr, 0, stream);
+}
+
+int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                            const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const void* rope_cos,
+                            const void* rope_sin, const void* k_tail, const void* v_tail, const int32_t* tail_len, int tail_cap,
+                            const uint32_t* v_lut, const float* signs, float sm_scale, int64_t window, int64_t sinks, void* workspace,
+                            size_t workspace_bytes, void* out, int out_dtype, void* stream) {
+  BMXK_REQUIRE(g != nullptr && g->layout == 1 && g->page == 128, "bmxk_k2b_decode_sliding: pools of layout 1 (128-token pages in row order) only");
+  BMXK_REQUIRE(window >= 1 && sinks >= 0, "bmxk_k2b_decode_sliding: window=%lld sinks=%lld (a query sees itself: window >= 1)", (long long)window,
+               (long long)sinks);
+  K2bWalk w = {};
+  w.tail_len = tail_cap > 0 ? tail_len : nullptr, w.tail_cap = tail_cap, w.window = window, w.sinks = sinks;
+  const int64_t most = (sinks + 127) / 128 + (window - 1) / 128 + 2;  // pages that hold a visible token
+  return decode_step(g, q, pages, coefs, basis_f16, page_table, table_stride, n_pages, batch, max_pages, rope_cos, rope_sin, 0, k_tail, v_tail,
+                     tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, nullptr, 3, WALK_SLIDING, w,
+                     most < max_pages ? (int)most : max_pages, nullptr, 0, stream);
+}
+
+size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split) {
+  if (!g || batch <= 0 || n_split <= 0) return 0;
+  const size_t own = (bmxk_k2b_decode_workspace_bytes(g, batch, 0) + 255) / 256 * 256;
+  return own + (size_t)batch * g->h_kv * g->n_q_groups * n_split * PREFIX_PART_STRIDE * sizeof(float);
+}
+
+int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
+                           const int32_t* members, const int32_t* group_start, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
+                           const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
+                           size_t workspace_bytes, void* out, int out_dtype, void* stream) {
+  BMXK_REQUIRE(g != nullptr && g->layout == 1 && g->page == 128, "bmxk_k2b_decode_shared: pools of layout 1 (128-token pages in row order) only");
+  BMXK_REQUIRE(g->h_kv >= 1 && g->h_kv <= 65535 && g->n_q_groups >= 1 && g->n_q_groups <= 8, "bmxk_k2b_decode_shared: h_kv=%d n_q_groups=%d", g->h_kv,
+               g->n_q_groups);
+  BMXK_REQUIRE(g->rank == 16 || g->rank == 32, "bmxk_k2b_decode_shared: rank=%d must be 16 or 32", g->rank);
+  BMXK_REQUIRE(g->group == 32 || g->group == 64 || g->group == 128, "bmxk_k2b_decode_shared: group=%d must be 32, 64 or 128", g->group);
+  BMXK_REQUIRE(g->n_coef_heads == 1 || g->n_coef_heads == g->h_kv, "bmxk_k2b_decode_shared: n_coef_heads=%d", g->n_coef_heads);
+  BMXK_REQUIRE(batch >= 1 && max_pages >= 0 && n_groups >= 0 && n_groups <= 65535 && max_members >= 0 && max_members <= batch,
+               "bmxk_k2b_decode_shared: batch=%d max_pages=%d n_groups=%d max_members=%d", batch, max_pages, n_groups, max_members);
+  BMXK_REQUIRE(n_split >= 1 && n_split <= 64, "bmxk_k2b_decode_shared: n_split=%d must be in 1..64", n_split);
+  BMXK_REQUIRE(skip && (n_groups == 0 || (members && group_start)), "bmxk_k2b_decode_shared: null group lists");
+  BMXK_REQUIRE(sm_scale > 0.f, "bmxk_k2b_decode_shared: sm_scale=%g must be positive", sm_scale);
+  BMXK_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= bmxk_k2b_decode_shared_workspace_bytes(g, batch, n_split),
+               "bmxk_k2b_decode_shared: workspace of %zu bytes needed (16-byte aligned), %zu given",
+               bmxk_k2b_decode_shared_workspace_bytes(g, batch, n_split), workspace_bytes);
+  const int bad = check_step(g, q, pages, coefs, basis_f16, page_table, n_pages, batch, max_pages, rope_cos, rope_sin, k_tail, v_tail, tail_len,
+                             tail_cap, v_lut, signs, workspace, workspace_bytes, out, out_dtype, nullptr, 3);
+  if (bad) return bad;
+  const bool prefixes = n_groups > 0 && max_members > 0 && max_pages > 0;
+  float* part = reinterpret_cast<float*>((uint8_t*)workspace + (bmxk_k2b_decode_workspace_bytes(g, batch, 0) + 255) / 256 * 256);
+  if (prefixes) {
+    BMXK_REQUIRE((((uintptr_t)q | (uintptr_t)pages | (uintptr_t)coefs | (uintptr_t)basis_f16 | (uintptr_t)rope_cos | (uintptr_t)rope_sin |
+                   (uintptr_t)rope_frag) & 15) == 0,
+                 "bmxk_k2b_decode_shared: q, pools, basis and rotation tables must be 16-byte aligned");
+    BMXK_REQUIRE(rope_frag == nullptr || rope_pages >= 1, "bmxk_k2b_decode_shared: rope_pages=%d", rope_pages);
+    PrefillParams prm = {};
+    prm.g.h_kv = g->h_kv, prm.g.n_q_groups = g->n_q_groups, prm.g.page = g->page, prm.g.rank = g->rank, prm.g.group = g->group;
+    prm.g.n_coef_heads = g->n_coef_heads, prm.g.kbits = g->kbits, prm.g.vbits = g->vbits, prm.g.layout = g->layout;
+    prm.q = (const __half*)q, prm.n_q = 1, prm.pages = (const uint8_t*)pages, prm.coefs = (const __half*)coefs;
+    prm.basis16 = (const __half*)basis_f16, prm.page_table = page_table, prm.table_stride = table_stride, prm.n_pages = n_pages;
+    prm.rope_cos = (const __half*)rope_cos, prm.rope_sin = (const __half*)rope_sin;
+    prm.rope_frag = (uint4*)rope_frag, prm.rope_pages = rope_frag ? rope_pages : 0;
+    prm.lut_lo = v_lut[0], prm.lut_hi = v_lut[1];
+    memcpy(&prm.lut_alpha, &v_lut[2], 4);
+    memcpy(&prm.lut_beta, &v_lut[3], 4);
+    prm.signs = signs, prm.scale_log2 = sm_scale * 1.4426950408889634f, prm.status = (int32_t*)workspace;
+    prm.n_split = n_split, prm.part = part, prm.skip = skip, prm.members = members, prm.group_start = group_start;
+    const int pp = 128 / g->n_q_groups;
+    const int rc = launch_prefix_t5(prm, dim3((unsigned)((max_members + pp - 1) / pp * n_split), (unsigned)g->h_kv, (unsigned)n_groups), (cudaStream_t)stream);
+    if (rc) return rc;
+  }
+  K2bWalk w = {};
+  w.skip = skip;
+  return decode_step(g, q, pages, coefs, basis_f16, page_table, table_stride, n_pages, batch, max_pages, rope_cos, rope_sin, 0, k_tail, v_tail,
+                     tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, nullptr, 3, WALK_OWN, w, max_pages,
+                     part, n_split, stream);
 }
 
 int bmxk_k2b_decode_static(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs,

@@ -85,7 +85,7 @@ __device__ __forceinline__ void named_bar(int id, int n) { asm volatile("bar.syn
 
 }  // namespace
 
-template <int RANK, int GQ>
+template <int RANK, int GQ, int WALK>
 __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bDecodeParams p) {
   constexpr int KS = RANK / 16;
   constexpr int COEF_BYTES = 128 * RANK * 2;
@@ -102,15 +102,30 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   uint8_t* pbuf0 = bbuf0 + 2 * COEF_BYTES;               // [2][4096] softmax weights per tile parity
   T5Smem* sh = reinterpret_cast<T5Smem*>(pbuf0 + 2 * T5_QB_BYTES);
   int* cum = reinterpret_cast<int*>(sh + 1);
-  int* npg_sm = cum + p.batch + 1;
+  int* npg_sm = cum + p.batch + 1;         // tiles of each sequence
+  int* gap_sm = npg_sm + p.batch;          // WALK_OWN, WALK_SLIDING: pages left out between tile keep - 1 and tile keep
+  int* first_sm = gap_sm + p.batch;        // WALK_SLIDING: first token of the window
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // the merge kernel is launched as this kernel's programmatic dependent: let its blocks become resident as soon as
   // SMs free up (it waits for this grid's completion itself before it reads the partial states)
   asm volatile("griddepcontrol.launch_dependents;");
-  if (warp == 0) fill_cum(cum, p.n_pages, p.batch, g.h_kv, 128, lane);
-  for (int i = tid; i < p.batch; i += T5_THREADS) npg_sm[i] = p.n_pages[i];
+  if constexpr (WALK == WALK_ALL) {
+    if (warp == 0) fill_cum(cum, p.n_pages, p.batch, g.h_kv, 128, lane);
+    for (int i = tid; i < p.batch; i += T5_THREADS) npg_sm[i] = p.n_pages[i];
+  } else {
+    for (int i = tid; i < p.batch; i += T5_THREADS) {
+      const PageSpan sp = page_span<WALK>(p.walk, p.n_pages[i], i);
+      npg_sm[i] = sp.tiles, gap_sm[i] = sp.gap;
+      if constexpr (WALK == WALK_SLIDING) first_sm[i] = (int)sp.first;
+    }
+    __syncthreads();
+    if (warp == 0) fill_cum(cum, npg_sm, p.batch, g.h_kv, 128, lane);
+  }
+  // page of tile j: where pages are left out behind the sinks, the sinks' pages are all there
+  const int keep = (WALK == WALK_SLIDING) ? (int)min((int64_t)0x7fffffff, (p.walk.sinks + 127) / 128) : 0;
+  auto page_of = [&](int b, int j) { return (WALK == WALK_ALL || j < keep) ? j : j + gap_sm[b]; };
   __syncthreads();
   const int total = cum[p.batch];
   const int per_cta = (total + gridDim.x - 1) / gridDim.x;
@@ -342,6 +357,15 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
 #pragma unroll
         for (int qi = 0; qi < GQ; ++qi) sv[qi] = __uint_as_float(r[qi]);
       }
+      bool hidden = false;  // this thread's token lies outside the window and is no sink: weight 0 whatever its score and norm are
+      if constexpr (WALK == WALK_SLIDING) {
+        const int t = page_of(w.cur.b, w.cur.j) * 128 + row;
+        hidden = t < first_sm[w.cur.b] && t >= p.walk.sinks;
+        if (hidden) {
+#pragma unroll
+          for (int qi = 0; qi < GQ; ++qi) sv[qi] = -INFINITY;
+        }
+      }
       // Lazy maximum: as long as no score of the tile exceeds the running maximum by more than 8 (weights
       // below 2^8), nothing is reduced; the four warps only exchange one flag each.
       bool need = false;
@@ -390,7 +414,8 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
         }
       }
       if (alive) {
-        const float norm = __half2float(reinterpret_cast<const __half*>(blk + k2b_off_vnorm(128, g.group))[row]);
+        float norm = __half2float(reinterpret_cast<const __half*>(blk + k2b_off_vnorm(128, g.group))[row]);
+        if (WALK == WALK_SLIDING && hidden) norm = 0.f;
         __half* pb = reinterpret_cast<__half*>(pbuf0 + (size_t)e * T5_QB_BYTES) + (row >> 3) * 64 + (row & 7);
 #pragma unroll
         for (int qi = 0; qi < GQ; qi += 2) {
@@ -490,7 +515,7 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
         const bool new_seg = (w.seg != prev_seg);
         if (new_seg) first_prev = first_cur, first_cur = w.it, prev_seg = w.seg;
         if ((w.it & 1) == rw) {
-          const int b = w.cur.b, h = w.cur.h, j = w.cur.j;
+          const int b = w.cur.b, h = w.cur.h, j = page_of(b, w.cur.j);
           const int64_t t0 = p.pos_offset + (int64_t)j * TILE_TOKENS;
           const __half* qsrc = p.q + ((int64_t)b * g.h_kv + h) * G * HEAD_DIM;
           // the page-table entry of this tile, for the copy warp: a global load there would sit in front of every
@@ -631,33 +656,39 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   }
 }
 
-static size_t t5_smem_bytes(int rank, int group, int batch) {
+static size_t t5_smem_bytes(int rank, int group, int batch, int walk) {
   const size_t coef = (size_t)128 * rank * 2;
   return (size_t)T5_STAGES * (coef + k2b_page_block_bytes(128, group)) + (size_t)(T5_STAGES + 2) * T5_QB_BYTES + 2 * coef +
-         sizeof(T5Smem) + (size_t)(2 * batch + 1) * 4 + 16;
+         sizeof(T5Smem) + (size_t)((walk == WALK_ALL ? 2 : 4) * batch + 1) * 4 + 16;
 }
 
-template <int RANK, int GQ>
+template <int RANK, int GQ, int WALK>
 static int launch_t5(const K2bDecodeParams& prm, int grid, size_t smem, cudaStream_t s) {
   static PerDeviceOnce configured;
   if (configured.first()) {
-    cudaError_t e = cudaFuncSetAttribute(k2b_decode_t5_kernel<RANK, GQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(k2b_decode_t5_kernel<RANK, GQ, WALK>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) {
       configured.retract();
       set_error("bmxk_k2b_decode: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return BMXK_ERR_CUDA;
     }
   }
-  k2b_decode_t5_kernel<RANK, GQ><<<grid, T5_THREADS, smem, s>>>(prm);
+  k2b_decode_t5_kernel<RANK, GQ, WALK><<<grid, T5_THREADS, smem, s>>>(prm);
   return check_launch("bmxk_k2b_decode(tcgen05)");
 }
-
-int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s) {
-  const size_t smem = t5_smem_bytes(prm.g.rank, prm.g.group, prm.batch);
-  BMXK_REQUIRE(smem <= 227 * 1024, "bmxk_k2b_decode: batch=%d too large for the tcgen05 kernel's shared memory", prm.batch);
+template <int WALK>
+static int launch_t5_walk(const K2bDecodeParams& prm, int grid, size_t smem, cudaStream_t s) {
   const bool g4 = prm.g.n_q_groups <= 4;
-  if (prm.g.rank == 32) return g4 ? launch_t5<32, 4>(prm, grid, smem, s) : launch_t5<32, 8>(prm, grid, smem, s);
-  return g4 ? launch_t5<16, 4>(prm, grid, smem, s) : launch_t5<16, 8>(prm, grid, smem, s);
+  if (prm.g.rank == 32) return g4 ? launch_t5<32, 4, WALK>(prm, grid, smem, s) : launch_t5<32, 8, WALK>(prm, grid, smem, s);
+  return g4 ? launch_t5<16, 4, WALK>(prm, grid, smem, s) : launch_t5<16, 8, WALK>(prm, grid, smem, s);
+}
+
+int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk) {
+  const size_t smem = t5_smem_bytes(prm.g.rank, prm.g.group, prm.batch, walk);
+  BMXK_REQUIRE(smem <= 227 * 1024, "bmxk_k2b_decode: batch=%d too large for the tcgen05 kernel's shared memory", prm.batch);
+  if (walk == WALK_OWN) return launch_t5_walk<WALK_OWN>(prm, grid, smem, s);
+  if (walk == WALK_SLIDING) return launch_t5_walk<WALK_SLIDING>(prm, grid, smem, s);
+  return launch_t5_walk<WALK_ALL>(prm, grid, smem, s);
 }
 
 }  // namespace bmxk

@@ -104,7 +104,8 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 }  // namespace
 
 // FRAG: the rotation tables of every page come from the rearranged copy (p.rope_frag)
-template <int RANK, bool FRAG>
+// MODE: what the 128 rows are and which keys they see (prefill_common.cuh)
+template <int RANK, bool FRAG, int MODE>
 __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const PrefillParams p) {
   constexpr int KS = RANK / 16;
   constexpr int COEF_BYTES = 128 * RANK * 2;
@@ -129,20 +130,32 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   const int n_split = p.n_split, share = (int)blockIdx.x % n_split, n_blocks = (int)gridDim.x / n_split;
   const int b = blockIdx.z, h = blockIdx.y, i0 = (n_blocks - 1 - (int)blockIdx.x / n_split) * PP;
   const int H = g.h_kv * G;
+  // MODE_PREFIX: row m is query head m % G of the group's member i0 + m / G (any G up to 8; 128 - PP * G rows idle)
+  const int m0 = MODE == MODE_PREFIX ? p.group_start[b] : 0, n_members = MODE == MODE_PREFIX ? p.group_start[b + 1] - m0 : 0;
+  if (MODE == MODE_PREFIX && i0 >= n_members) return;
+  const int first_member = MODE == MODE_PREFIX ? p.members[m0] : b;
 
   const int64_t pq_min = p.q_pos0 + i0;                                // first query position of the CTA
   const int64_t pq_max = p.q_pos0 + min(i0 + PP, p.n_q) - 1;           // last one
-  const int n_pg = p.n_pages[b];
-  const int64_t vis = pq_max - p.pos_offset;
-  const int NPv = (vis < 0) ? 0 : (int)min((int64_t)(FRAG ? min(n_pg, p.rope_pages) : n_pg), vis / 128 + 1);  // pages whose first token the last position sees
+  const int n_pg = MODE == MODE_PREFIX ? min(max(p.skip[first_member], 0), p.n_pages[first_member]) : p.n_pages[b];
+  const int64_t vis = MODE == MODE_PREFIX ? (int64_t)n_pg * 128 : pq_max - p.pos_offset;
+  if (MODE != MODE_CAUSAL && FRAG && tid == 0 && min((int64_t)n_pg, vis / 128 + 1) > p.rope_pages && atomicCAS(p.status, 0, 3) == 0)
+    p.status[1] = p.rope_pages, p.status[2] = n_pg;
+  const int n_last = (vis < 0) ? 0 : (int)min((int64_t)(FRAG ? min(n_pg, p.rope_pages) : n_pg), vis / 128 + 1);  // pages whose first token the last position sees
+  // MODE_SLIDING: of those, the sinks' pages [0, keep) and the pages from the first row's window on; the gap between them is left out
+  const int64_t lo_min = MODE == MODE_SLIDING ? max((int64_t)0, pq_min - p.window + 1) : 0, lo_max = MODE == MODE_SLIDING ? pq_max - p.window + 1 : 0;
+  const int keep = MODE == MODE_SLIDING ? (int)min((int64_t)n_last, (p.sinks + 127) / 128) : 0;
+  const int gap = MODE == MODE_SLIDING ? max(0, (int)min((int64_t)n_last, lo_min / 128) - keep) : 0;
+  const int NPv = n_last - gap;
   // this CTA's share of them: pages T0 .. T0 + NP - 1; the window goes with the last share
   const int per_share = (NPv + n_split - 1) / n_split;
   const int T0 = min(NPv, share * per_share), NP = min(NPv, T0 + per_share) - T0;
-  const int tl = p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
+  auto page_of = [&](int n) { return MODE == MODE_SLIDING && T0 + n >= keep ? T0 + n + gap : T0 + n; };  // page of this share's tile n
+  const int tl = MODE == MODE_PREFIX ? 0 : p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
   const int64_t tail_pos0 = p.pos_offset + (int64_t)n_pg * 128;
   const int NW = (share == n_split - 1 && tl > 0 && pq_max >= tail_pos0) ? (int)((min((int64_t)tl, pq_max - tail_pos0 + 1) + 127) / 128) : 0;
   const int NT = NP + NW;
-  const int64_t page_pos0 = p.pos_offset + (int64_t)T0 * 128;  // position of the first key of this share
+  const int64_t page_pos0 = p.pos_offset + (int64_t)T0 * 128;  // position of the first key of this share (MODE_SLIDING: see page_of)
 
   // ---- prologue: barriers, tensor memory, the operands that do not change (Q, basis, constant rows of V') ----
   if (tid == 0) {
@@ -159,9 +172,12 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   }
   for (int o = tid; o < 128 * 18; o += P5_THREADS) {  // row m = (query head m / PP, position i0 + m % PP)
     const int m = o / 18, c8 = o % 18;
-    const int qi = m / PP, ip = min(i0 + m % PP, p.n_q - 1);
+    const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
     uint4 v = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
-    if (c8 < 16) v = reinterpret_cast<const uint4*>(p.q + (((int64_t)b * H + h * G + qi) * p.n_q + ip) * HEAD_DIM)[c8];
+    if (c8 < 16) {
+      const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+      v = reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM)[c8];
+    }
     *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = v;
     if (c8 == 17) {  // K index 136 .. 143 of both key buffers: zero for good
       *reinterpret_cast<uint4*>(kop0 + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -203,14 +219,14 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     // chunk are reloaded for the next tile as soon as the chunk is done, so the loads have a whole tile to land.
     // From the tables themselves a warp's load touches 32 rows of 256 bytes; from the rearranged copy it is 512 bytes on end.
     uint4 cs4[2][2], sn4[2][2];
-    const uint4* frag0 = FRAG ? p.rope_frag + (int64_t)T0 * ROPE_FRAG_UINT4 + (k0 * 4 + wq) * 64 + lane : nullptr;
+    const uint4* frag0 = FRAG ? p.rope_frag + (MODE == MODE_SLIDING ? 0 : (int64_t)T0 * ROPE_FRAG_UINT4) + (k0 * 4 + wq) * 64 + lane : nullptr;
     auto load_rope = [&](int n, int kk) {
       if constexpr (FRAG) {
-        const uint4* pc = frag0 + (int64_t)n * ROPE_FRAG_UINT4 + kk * 256;
+        const uint4* pc = frag0 + (int64_t)(MODE == MODE_SLIDING ? page_of(n) : n) * ROPE_FRAG_UINT4 + kk * 256;
         const uint4* ps = pc + ROPE_FRAG_UINT4 / 2;
         cs4[kk][0] = pc[0], cs4[kk][1] = pc[32], sn4[kk][0] = ps[0], sn4[kk][1] = ps[32];
       } else {
-        const int64_t pos = page_pos0 + (int64_t)n * 128 + row;
+        const int64_t pos = MODE == MODE_SLIDING ? p.pos_offset + (int64_t)page_of(n) * 128 + row : page_pos0 + (int64_t)n * 128 + row;
         const uint4* pc = reinterpret_cast<const uint4*>(p.rope_cos + pos * HEAD_DIM + 16 * (k0 + kk));
         const uint4* ps = reinterpret_cast<const uint4*>(p.rope_sin + pos * HEAD_DIM + 16 * (k0 + kk));
         cs4[kk][0] = pc[0], cs4[kk][1] = pc[1], sn4[kk][0] = ps[0], sn4[kk][1] = ps[1];
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       } else {
         // window tile: the keys are stored rotated; rows past the window's length are zero; norm 1
         const int t0 = (n - NP) * 128;
-        const bool valid = t0 + row < tl;
+        const bool valid = t0 + row < tl && (MODE != MODE_SLIDING || tail_pos0 + t0 + row >= lo_min || tail_pos0 + t0 + row < p.sinks);
         const uint4* src = reinterpret_cast<const uint4*>(kt + (int64_t)(t0 + row) * HEAD_DIM);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -368,8 +384,10 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int ta = t0 + 64 * cc + 8 * i + 2 * j;
-            const __half a = (ta < tl) ? vt[(int64_t)ta * HEAD_DIM + ch] : __float2half_rn(0.f);
-            const __half c = (ta + 1 < tl) ? vt[(int64_t)(ta + 1) * HEAD_DIM + ch] : __float2half_rn(0.f);
+            // (MODE_SLIDING: what no row of the block sees stays out, so that no infinity in it meets a weight of 0)
+            auto in = [&](int t) { return t < tl && (MODE != MODE_SLIDING || tail_pos0 + t >= lo_min || tail_pos0 + t < p.sinks); };
+            const __half a = in(ta) ? vt[(int64_t)ta * HEAD_DIM + ch] : __float2half_rn(0.f);
+            const __half c = in(ta + 1) ? vt[(int64_t)(ta + 1) * HEAD_DIM + ch] : __float2half_rn(0.f);
             w4[j] = h2_as_u32(__halves2half2(a, c));
           }
           *reinterpret_cast<uint4*>(vrow + (8 * cc + i) * 128) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
@@ -391,7 +409,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P5_REG_SOFTMAX));
     const int wq = warp & 3, row = 32 * wq + lane, hf = (warp - 8) >> 2;
     const uint32_t tl_ = tmem + ((uint32_t)(32 * wq) << 16);
-    const int qi = row / PP, ip = i0 + row % PP;
+    const int qi = MODE == MODE_PREFIX ? row % G : row / PP, ip = MODE == MODE_PREFIX ? i0 + row / G : i0 + row % PP;
     const int64_t pq = p.q_pos0 + ip;
     float m = -1e30f;
     bool alive = true;
@@ -474,10 +492,15 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     for (int n = 0; n < NT && alive; ++n) {  // half tile u = (tile n, half hf): tokens 64 hf .. 64 hf + 63
       const int u = 2 * n + hf, e = n & 1;
       // keys of the half visible to this row / to the CTA's first row: position - first key position + 1
-      const int64_t key0 = (n < NP ? page_pos0 + (int64_t)n * 128 : tail_pos0 + (int64_t)(n - NP) * 128) + 64 * hf;
+      const int64_t key0 = (n < NP ? (MODE == MODE_SLIDING ? p.pos_offset + (int64_t)page_of(n) * 128 : page_pos0 + (int64_t)n * 128)
+                                   : tail_pos0 + (int64_t)(n - NP) * 128) + 64 * hf;
       const int64_t rel = pq - key0 + 1, rel_min = pq_min - key0 + 1;
       const int n_valid = (n < NP) ? 64 : max(0, min(64, tl - (n - NP) * 128 - 64 * hf));
-      const bool masked = (rel_min < 64) || (n_valid < 64);                               // the same for the whole CTA
+      const bool masked = MODE != MODE_PREFIX && ((rel_min < 64) || (n_valid < 64) ||
+                                                  (MODE == MODE_SLIDING && key0 < lo_max && key0 + 64 > p.sinks));  // the same for the whole CTA
+      // MODE_SLIDING: of the half's keys this row sees [0, js) as sinks and [jw, jl) as its window
+      const int js = MODE == MODE_SLIDING ? (int)max((int64_t)0, min((int64_t)64, p.sinks - key0)) : 0;
+      const int jw = MODE == MODE_SLIDING ? (int)max((int64_t)0, min((int64_t)64, pq - p.window + 1 - key0)) : 0;
       const int jl = (int)max((int64_t)0, min((int64_t)n_valid, rel));                    // keys [0, jl) of the half are visible to this row
       const uint32_t tS = tl_ + TM_S + 64 * hf, tP = tl_ + TM_P + 32 * hf;
       if (hf == 0 && n == NP && NP > 0) {  // first window tile after pages: leave the rotated space of the value codec
@@ -504,8 +527,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       if (masked) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          ra[i] = i < jl ? ra[i] : 0xFF800000u;  // -inf: weight 0
-          rb[i] = 32 + i < jl ? rb[i] : 0xFF800000u;
+          ra[i] = i < jl && (MODE != MODE_SLIDING || i >= jw || i < js) ? ra[i] : 0xFF800000u;  // -inf: weight 0
+          rb[i] = 32 + i < jl && (MODE != MODE_SLIDING || 32 + i >= jw || 32 + i < js) ? rb[i] : 0xFF800000u;
         }
       }
       float t4[4];
@@ -575,7 +598,38 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     // ---- the last U3, the rotation if no window tile undid it, normalise and store ----
     if (alive && NT > 0 && !(warp_wait(&sh->odone[0], (uint32_t)(NT - 1) & 1u, p.status, 49) && warp_wait(&sh->odone[1], (uint32_t)(NT - 1) & 1u, p.status, 49)))
       alive = false;
-    if (alive) {
+    if (MODE == MODE_PREFIX && alive) {
+      // record of this share: accumulators as the value table's affine map leaves them (the rotation is undone where the parts are
+      // merged), running maximum, sum of weights
+      const bool live = row < PP * G && ip < n_members;
+      float* rec = p.part + (((int64_t)(live ? p.members[m0 + ip] : 0) * H + h * G + qi) * n_split + share) * PREFIX_PART_STRIDE;
+      float lsum = 0.f, add = 0.f;
+      if (NT > 0) {
+        tc5::fence_after();
+        uint32_t r4[4];
+        tc5::ld4(tl_ + TM_O + 128, r4);
+        tc5::wait_ld();
+        lsum = __uint_as_float(r4[0]) + __uint_as_float(r4[1]), add = p.lut_alpha * __uint_as_float(r4[2]);
+      }
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r[32];
+        if (NT > 0) {
+          tc5::ld32(tl_ + TM_O + 32 * c, r);
+          tc5::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(p.lut_beta, __uint_as_float(r[i]), add));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(rec + 32 * c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        }
+      }
+      if (live) *reinterpret_cast<float4*>(rec + 128) = make_float4(NT > 0 ? m : -INFINITY, lsum, 0.f, 0.f);
+    } else if (alive) {
       float inv = 0.f;
       if (NT > 0) {
         tc5::fence_after();
@@ -667,10 +721,10 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       constexpr uint32_t ID_U1 = tc5::idesc_f16_f16(128, 128);
       const uint64_t d_stage = tc5::smem_desc(smem_u32(stage0), 128, AB_SBO), d_b = tc5::smem_desc(smem_u32(bop), 128, AB_SBO);
       const int chd = (g.n_coef_heads == 1) ? 0 : h;
-      const int32_t* table = p.page_table + (int64_t)b * p.table_stride + T0;
+      const int32_t* table = p.page_table + (int64_t)first_member * p.table_stride;
       int nP = 0, nA = 0, sP = 0, sA = 0;
       uint32_t phA = 0;
-      int slot = (NP > 0) ? table[0] : 0;  // page slot of the next copy, fetched one copy ahead
+      int slot = (NP > 0) ? table[page_of(0)] : 0;  // page slot of the next copy, fetched one copy ahead
       while (ok && nA < NP) {
         bool progressed = false;
         const int kc0 = smem_load_acquire(&sh->kcnt[0]), kc1 = smem_load_acquire(&sh->kcnt[1]);
@@ -704,7 +758,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
           __syncwarp();
           ++nP;
           if (++sP == P5_STAGES) sP = 0;
-          if (nP < NP) slot = table[nP];
+          if (nP < NP) slot = table[page_of(nP)];
           progressed = true;
         }
         if (stalled(progressed, 40)) ok = false;
@@ -770,18 +824,18 @@ static size_t p5_smem_bytes(int rank, int group) {
          (size_t)128 * rank * 2 + 128 * 4 + sizeof(P5Smem) + 128;
 }
 
-template <int RANK, bool FRAG>
+template <int RANK, bool FRAG, int MODE>
 static int launch_p5(const PrefillParams& prm, dim3 grid, size_t smem, cudaStream_t s) {
   static PerDeviceOnce configured;
   if (configured.first()) {
-    cudaError_t e = cudaFuncSetAttribute((k2b_prefill_t5_kernel<RANK, FRAG>), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    cudaError_t e = cudaFuncSetAttribute((k2b_prefill_t5_kernel<RANK, FRAG, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) {
       configured.retract();
       set_error("bmxk_k2b_prefill: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return BMXK_ERR_CUDA;
     }
   }
-  k2b_prefill_t5_kernel<RANK, FRAG><<<grid, P5_THREADS, smem, s>>>(prm);
+  k2b_prefill_t5_kernel<RANK, FRAG, MODE><<<grid, P5_THREADS, smem, s>>>(prm);
   return check_launch("bmxk_k2b_prefill(tcgen05)");
 }
 
@@ -821,6 +875,34 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(const float* __restr
   out[row * HEAD_DIM + threadIdx.x] = __float2half_rn(l > 0.f ? acc / l : 0.f);
 }
 
+static int merge_shares(const PrefillParams& prm, dim3 grid, cudaStream_t s) {
+  if (prm.n_split <= 1) return BMXK_OK;
+  const int64_t rows = (int64_t)grid.z * prm.g.h_kv * prm.g.n_q_groups * prm.n_q;
+  prefill_merge_kernel<<<(unsigned)rows, 128, 0, s>>>(prm.part, prm.n_split, prm.out);
+  return check_launch("bmxk_k2b_prefill(merge)");
+}
+
+template <int MODE>
+static int launch_p5_mode(const PrefillParams& prm, dim3 grid, cudaStream_t s) {
+  const size_t smem = p5_smem_bytes(prm.g.rank, prm.g.group);
+  BMXK_REQUIRE(smem <= 227 * 1024, "bmxk_k2b_prefill: rank=%d group=%d needs %zu bytes of shared memory", prm.g.rank, prm.g.group, smem);
+  if (prm.rope_frag) return prm.g.rank == 32 ? launch_p5<32, true, MODE>(prm, grid, smem, s) : launch_p5<16, true, MODE>(prm, grid, smem, s);
+  return prm.g.rank == 32 ? launch_p5<32, false, MODE>(prm, grid, smem, s) : launch_p5<16, false, MODE>(prm, grid, smem, s);
+}
+
+int launch_prefill_t5_sliding(const PrefillParams& prm, dim3 grid, cudaStream_t s) {
+  const int rc = launch_p5_mode<MODE_SLIDING>(prm, grid, s);
+  return rc ? rc : merge_shares(prm, grid, s);
+}
+
+int launch_prefix_t5(const PrefillParams& prm, dim3 grid, cudaStream_t s) { return launch_p5_mode<MODE_PREFIX>(prm, grid, s); }
+
+// Rotation tables of n_pages pages from position 0 on, in the order of the key warps' reads: kept by callers that attend often.
+int launch_rope_fragments(const __half* rope_cos, const __half* rope_sin, uint4* frag, int n_pages, cudaStream_t s) {
+  rope_fragments_kernel<<<(unsigned)n_pages * 8, 256, 0, s>>>(rope_cos, rope_sin, 0, frag, n_pages, nullptr, 0, -1, nullptr);
+  return check_launch("bmxk_k2b_rope_fragments");
+}
+
 int launch_prefill_t5(const PrefillParams& prm, dim3 grid, cudaStream_t s) {
   const size_t smem = p5_smem_bytes(prm.g.rank, prm.g.group);
   BMXK_REQUIRE(smem <= 227 * 1024, "bmxk_k2b_prefill: rank=%d group=%d needs %zu bytes of shared memory", prm.g.rank, prm.g.group, smem);
@@ -830,14 +912,11 @@ int launch_prefill_t5(const PrefillParams& prm, dim3 grid, cudaStream_t s) {
                                                                               prm.n_pages, (int)grid.z, prm.q_pos0 + prm.n_q - 1, prm.status);
     rc = check_launch("bmxk_k2b_prefill(rope fragments)");
     if (rc) return rc;
-    rc = prm.g.rank == 32 ? launch_p5<32, true>(prm, grid, smem, s) : launch_p5<16, true>(prm, grid, smem, s);
+    rc = prm.g.rank == 32 ? launch_p5<32, true, MODE_CAUSAL>(prm, grid, smem, s) : launch_p5<16, true, MODE_CAUSAL>(prm, grid, smem, s);
   } else {
-    rc = prm.g.rank == 32 ? launch_p5<32, false>(prm, grid, smem, s) : launch_p5<16, false>(prm, grid, smem, s);
+    rc = prm.g.rank == 32 ? launch_p5<32, false, MODE_CAUSAL>(prm, grid, smem, s) : launch_p5<16, false, MODE_CAUSAL>(prm, grid, smem, s);
   }
-  if (rc != BMXK_OK || prm.n_split <= 1) return rc;
-  const int64_t rows = (int64_t)grid.z * prm.g.h_kv * prm.g.n_q_groups * prm.n_q;
-  prefill_merge_kernel<<<(unsigned)rows, 128, 0, s>>>(prm.part, prm.n_split, prm.out);
-  return check_launch("bmxk_k2b_prefill(merge)");
+  return rc ? rc : merge_shares(prm, grid, s);
 }
 
 }  // namespace bmxk

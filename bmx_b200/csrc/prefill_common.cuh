@@ -37,12 +37,27 @@ struct PrefillParams {
   // rope_fragments_kernel), or null: the tables are read where they are.
   uint4* rope_frag;
   int rope_pages;
+  // MODE_SLIDING: a row at position x sees the keys of (x - window, x] and those below `sinks`; pages that no row of a block sees are
+  // not touched
+  int64_t window, sinks;
+  // MODE_PREFIX: single-token queries q (batch, heads, 128) of the sequences members[group_start[z] .. group_start[z + 1] - 1] over
+  // the first skip[first member] pages of the first member's page-table row, which all of them share
+  const int32_t* skip;
+  const int32_t* members;
+  const int32_t* group_start;
 };
+constexpr int MODE_CAUSAL = 0, MODE_PREFIX = 1, MODE_SLIDING = 2;
 constexpr int ROPE_FRAG_UINT4 = 2048;  // per page: [cos, sin][chunk of 16 pairs][32 tokens x 4][half of the chunk][lane]
 constexpr int PF_PART_STRIDE = 132;  // floats per (row, share) record: 16-byte aligned rows
 
 // tcgen05 prefill kernel (k2b_prefill_t5.cu); the mma.sync kernel's grid with x multiplied by n_split.  Needs q, out and the
 // window 16-byte aligned.  With n_split > 1 the merge kernel is launched behind it.
 int launch_prefill_t5(const PrefillParams& prm, dim3 grid, cudaStream_t s);
+// The same kernel under a sliding window (grid and merge as above; rope_frag holds rearranged tables already, or is null).
+int launch_prefill_t5_sliding(const PrefillParams& prm, dim3 grid, cudaStream_t s);
+// The shared-prefix part of a decode step: grid (blocks of 128 / n_q_groups sequences x n_split, h_kv, groups), records of
+// PREFIX_PART_STRIDE floats to prm.part[(sequence, query head)][n_split], value rotation not undone.
+int launch_prefix_t5(const PrefillParams& prm, dim3 grid, cudaStream_t s);
+int launch_rope_fragments(const __half* rope_cos, const __half* rope_sin, uint4* frag, int n_pages, cudaStream_t s);
 
 }  // namespace bmxk

@@ -59,12 +59,22 @@ def dequant_value_blocks(vpool: torch.Tensor, slots: torch.Tensor, codebook: tor
 class K2bLayerState:
     """Packed pages + fp16 recent window of one layer for `batch` sequences of equal length."""
 
+    # A query sees the last sliding_window tokens (itself among them) and the first `sinks`; None: everything.
+    sliding_window: int | None = None
+    sinks = 0
+
     # callable (k_src, n_pages) -> (batch, n_pages * page, rank) float32 that replaces the append kernel's own projection
     # (a basis spanning heads that other GPUs hold: dist.HeadShardedK2bLayer); None: the kernel projects
     project = None
 
     def __init__(self, geom, batch: int, max_tokens: int, recent_window: int, device, rope_cos: torch.Tensor,
-                 rope_sin: torch.Tensor, *, codebook=None, v_seed: int = 0, pre_rope: bool = True):
+                 rope_sin: torch.Tensor, *, codebook=None, v_seed: int = 0, pre_rope: bool = True, sliding_window: int | None = None,
+                 sinks: int = 0):
+        if sliding_window is not None and (sliding_window < 1 or sinks < 0 or geom.layout != 1 or not pre_rope):
+            raise ValueError(f"sliding_window={sliding_window}, sinks={sinks}: a window of at least one token over 128-token pages of layout 1")
+        if sliding_window is None and sinks:
+            raise ValueError("sinks without a sliding_window: every token is visible already")
+        self.sliding_window, self.sinks = sliding_window, sinks
         assert rope_cos.dtype == torch.float16 and rope_cos.shape[1] == HEAD_DIM and rope_cos.shape[0] >= 128
         self.geom, self.batch, self.device = geom, batch, torch.device(device)
         self.page, self.W, self.pre_rope = geom.page, recent_window, pre_rope
@@ -203,6 +213,12 @@ class K2bLayerState:
         """q (batch, heads, 128) fp16 -> attention output (batch, heads, 128) over pages + window.  pos_offset: rotary
         position of this state's first committed token (a rank that holds a later part of a split sequence)."""
         max_pages = self.max_pages if self.committed else 0  # nothing committed yet: window only
+        if self.sliding_window is not None:
+            if partial_out is not None or phases != 3 or pos_offset:
+                raise NotImplementedError("a sliding window decodes in one piece: no partial states, phases or position offsets")
+            return K.k2b_decode_sliding(self.pool, q, self.basis_f16, self.page_table, self.n_pages_dev, max_pages, self.rope_cos, self.rope_sin,
+                                        self.k_win, self.v_win, self.tail_len_dev, self.v_lut, self.signs, self.sm_scale, self.workspace,
+                                        self.sliding_window, self.sinks, out=out)
         return K.k2b_decode(self.pool, q, self.basis_f16, self.page_table, self.n_pages_dev, max_pages,
                             self.rope_cos, self.rope_sin, self.k_win, self.v_win, self.tail_len_dev, self.v_lut,
                             self.signs, self.sm_scale, self.workspace, out=out, partial_out=partial_out, pos_offset=pos_offset,
@@ -214,6 +230,19 @@ class K2bLayerState:
         :320-395).  Returns None when this state has no such kernel (64-token pages): the caller takes the dense route."""
         if type(self) is not K2bLayerState or self.geom.layout != 1 or self.geom.n_q_groups not in (1, 2, 4, 8):
             return None
+        if self.sliding_window is not None:
+            last = max(0, q_pos0 + q.shape[2] - 1) // self.page + 1
+            seen = min(last, (self.sliding_window + q.shape[2]) // self.page + 2 + -(-self.sinks // self.page))
+            blocks = -(-q.shape[2] // (128 // self.geom.n_q_groups)) * self.geom.h_kv * self.batch
+            rope = None
+            if blocks * seen >= self.ROPE_FRAGMENT_TILES * _sm_count(self.device) and self.rope_cos.shape[0] >= last * self.page:
+                rope = K.rope_fragments(self.rope_cos, self.rope_sin, last)
+            basis16 = self.basis_f16
+            if basis16 is None:  # nothing committed yet: the kernel reads no page
+                basis16 = torch.zeros(self.geom.h_kv * HEAD_DIM, self.geom.rank, dtype=torch.float16, device=self.device)
+            return K.k2b_prefill_sliding(self.pool, q, q_pos0, basis16, self.page_table, self.n_pages_dev, self.max_pages, self.rope_cos,
+                                         self.rope_sin, rope, self.k_win, self.v_win, self.tail_len_dev, self.v_lut, self.signs, self.sm_scale,
+                                         self.workspace, self.sliding_window, self.sinks, out=out)
         return K.k2b_prefill(self.pool, q, q_pos0, self.basis_f16, self.page_table, self.n_pages_dev, self.rope_cos, self.rope_sin,
                              self.k_win, self.v_win, self.tail_len_dev, self.v_lut, self.signs, self.sm_scale,
                              self.workspace.view(torch.int32), out=out, n_split=self.prefill_split(q.shape[2]),

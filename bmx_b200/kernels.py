@@ -6,6 +6,7 @@ libbmxk.so and raises `BmxkError` on a non-zero status.  Nothing in this module 
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import struct
@@ -62,6 +63,16 @@ def _require_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("bmxk kernels take CUDA tensors; there is no CPU path")
+
+
+def _on_device_of(*ts: torch.Tensor | None):
+    """The context in which a call on these tensors runs: their device, one for all of them, made current if it is not."""
+    _require_cuda(*ts)
+    devices = {t.device.index for t in ts if t is not None}
+    if len(devices) != 1:
+        raise RuntimeError(f"tensors of one call lie on different devices: {sorted(devices)}")
+    index = devices.pop()
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _require_device_visible(*ts: torch.Tensor) -> None:
@@ -311,6 +322,183 @@ def k2b_prefill(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: torch.Te
     return out
 
 
+# ---- sliding windows and shared prefixes ----------------------------------------------------------
+
+
+def rope_fragments(rope_cos: torch.Tensor, rope_sin: torch.Tensor, n_pages: int) -> torch.Tensor:
+    """The rotation tables of the first n_pages 128-token pages in the order in which the prefill kernel reads them (int32
+    (n_pages, 8192), 32 KB per page), made once and kept next to the tables by callers that attend often."""
+    assert rope_cos.dtype == rope_sin.dtype == torch.float16 and rope_cos.dim() == 2 and rope_cos.shape[1] == rope_sin.shape[1] == HEAD_DIM
+    assert rope_cos.is_contiguous() and rope_sin.is_contiguous()
+    assert n_pages >= 1 and 128 * n_pages <= min(rope_cos.shape[0], rope_sin.shape[0]), "rotation tables end before the pages asked for"
+    with _on_device_of(rope_cos, rope_sin):
+        frag = torch.empty(n_pages, int(_lib.lib().bmxk_k2b_prefill_rope_bytes(1)) // 4, dtype=torch.int32, device=rope_cos.device)
+        call("bmxk_k2b_rope_fragments", _ptr(rope_cos), _ptr(rope_sin), int(n_pages), _ptr(frag), _stream())
+    return frag
+
+
+@functools.lru_cache(maxsize=None)
+def _sm_count(device: torch.device) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def split_walk(ctas: int, pages: int, device, most: int = 64) -> int:
+    """Shares of a page walk of `pages` pages that `ctas` CTAs would each make whole: the number that makes (waves of CTAs) x (pages
+    per share + the CTA's set-up, about four pages' worth) smallest."""
+    n_sm = _sm_count(torch.device(device))
+    best, best_cost = 1, None
+    for s in range(1, max(1, min(most, pages)) + 1):
+        cost = -(-ctas * s // n_sm) * (-(-pages // s) + 4)
+        if best_cost is None or cost < best_cost:
+            best, best_cost = s, cost
+    return best
+
+
+def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int, basis_f16: torch.Tensor | None,
+                rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, k_tail: torch.Tensor | None, v_tail: torch.Tensor | None,
+                tail_len: torch.Tensor | None, signs: torch.Tensor) -> int:
+    """What every step over a k2b pool asks of its tensors; returns the window's capacity."""
+    g = pool.geom
+    batch = q.shape[0]
+    assert q.dtype == torch.float16 and q.is_contiguous() and q.shape[1] == g.h_kv * g.n_q_groups and q.shape[-1] == HEAD_DIM
+    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == batch and page_table.stride(1) == 1
+    assert n_pages.dtype == torch.int32 and n_pages.shape == (batch,) and n_pages.is_contiguous()
+    assert 0 <= max_pages <= page_table.shape[1], f"max_pages={max_pages}: the page table has {page_table.shape[1]} columns"
+    assert signs.dtype == torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
+    if max_pages > 0:
+        assert basis_f16.dtype == torch.float16 and basis_f16.shape == (g.h_kv * HEAD_DIM, g.rank) and basis_f16.is_contiguous()
+        for t in (rope_cos, rope_sin):
+            assert t.dtype == torch.float16 and t.is_contiguous() and t.shape[1] == HEAD_DIM and t.shape[0] >= 128
+    if k_tail is None:
+        assert v_tail is None and tail_len is None
+        return 0
+    tail_cap = k_tail.shape[2]
+    assert k_tail.dtype == v_tail.dtype == torch.float16 and k_tail.is_contiguous() and v_tail.is_contiguous()
+    assert k_tail.shape == (batch, g.h_kv, tail_cap, HEAD_DIM) == v_tail.shape
+    assert tail_len.dtype == torch.int32 and tail_len.shape == (batch,) and tail_len.is_contiguous()
+    return tail_cap
+
+
+def _check_out(out: torch.Tensor | None, q: torch.Tensor, dtypes: tuple) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=torch.float16, device=q.device)
+    _require_device_visible(out)
+    assert out.dtype in dtypes and out.is_contiguous() and out.shape == q.shape
+    return out
+
+
+def k2b_decode_sliding(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int,
+                       rope_cos: torch.Tensor, rope_sin: torch.Tensor, k_tail: torch.Tensor | None, v_tail: torch.Tensor | None,
+                       tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor, sm_scale: float, workspace: torch.Tensor,
+                       window: int, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """k2b_decode under a sliding window: the newest token sees the last `window` tokens held (itself among them) and the first
+    `sinks`.  Pages in between are not read; their page-table entries may be anything.  Layout 1.  A sequence that holds nothing gives 0.
+    workspace: decode_workspace()."""
+    g = pool.geom
+    assert q.dim() == 3
+    with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs, workspace):
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        out = _check_out(out, q, (torch.float16, torch.float32))
+        call("bmxk_k2b_decode_sliding", ctypes.byref(g), _ptr(q), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16), _ptr(page_table),
+             page_table.stride(0), _ptr(n_pages), q.shape[0], max_pages, _ptr(rope_cos), _ptr(rope_sin), _ptr(k_tail), _ptr(v_tail), _ptr(tail_len),
+             tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), int(window), int(sinks), _ptr(workspace), workspace.numel(), _ptr(out),
+             _dtype_code(out), _stream())
+    return out
+
+
+def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor,
+                        max_pages: int, rope_cos: torch.Tensor, rope_sin: torch.Tensor, rope: torch.Tensor | None, k_tail: torch.Tensor | None,
+                        v_tail: torch.Tensor | None, tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor, sm_scale: float,
+                        status: torch.Tensor, window: int, sinks: int = 0, out: torch.Tensor | None = None, n_split: int | None = None) -> torch.Tensor:
+    """k2b_prefill under a sliding window: row i of q (batch, heads, n_q, 128) fp16 stands at position x = q_pos0 + i and sees the
+    keys in (x - window, x] and the first `sinks` up to x.  Pages that no row sees are not read.  rope: rope_fragments() of every page held
+    up to the last row's position (too few are reported in the status word), or None (the tables are read as they are).  status: zeroed device memory (a decode workspace serves).  n_split: shares of
+    a block's page walk, by default what fills the GPU."""
+    g = pool.geom
+    assert q.dim() == 4 and q.shape[2] >= 1
+    batch, n_q = q.shape[0], q.shape[2]
+    with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, status):
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        assert status.numel() * status.element_size() >= 16 and status.is_contiguous()
+        rope_pages = _check_fragments(rope, 0)
+        out = _check_out(out, q, (torch.float16,))
+        if n_split is None:
+            pp = max(1, 128 // g.n_q_groups)
+            seen = min(max_pages, -(-sinks // g.page) + (window + min(pp, n_q)) // g.page + 2)
+            ctas = -(-n_q // pp) * g.h_kv * batch
+            n_split = split_walk(ctas, seen, q.device, 16)
+        nbytes = int(_lib.lib().bmxk_k2b_prefill_workspace_bytes(ctypes.byref(g), n_q, batch, int(n_split)))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        call("bmxk_k2b_prefill_sliding", ctypes.byref(g), _ptr(q), n_q, int(q_pos0), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16),
+             _ptr(page_table), page_table.stride(0), _ptr(n_pages), batch, _ptr(rope_cos), _ptr(rope_sin), _ptr(rope), rope_pages, _ptr(k_tail),
+             _ptr(v_tail), _ptr(tail_len), tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), int(window), int(sinks), _ptr(status),
+             _ptr(out), int(n_split), _ptr(ws), nbytes, _stream())
+    return out
+
+
+def _check_fragments(rope: torch.Tensor | None, pages: int) -> int:
+    if rope is None:
+        return 0
+    assert rope.dtype == torch.int32 and rope.dim() == 2 and rope.shape[1] == 8192 and rope.is_contiguous(), "rope: rope_fragments()"
+    assert rope.shape[0] >= pages, f"rotation tables rearranged for {rope.shape[0]} pages, {pages} are shared"
+    return rope.shape[0]
+
+
+class PrefixGroups:
+    """Which sequences of a batch share a prefix of whole pages, for k2b_decode_shared: members[i] lists the batch rows of group i and
+    prefix_pages[i] how many of the first entries of their page-table rows are the same pages.  Rows in no group are decoded as by
+    k2b_decode.  One small host-to-device copy; the object can be used for as many steps as the grouping lasts."""
+
+    def __init__(self, g: K2bGeom, batch: int, members: list, prefix_pages: list, device, n_split: int | None = None):
+        assert batch >= 1 and len(members) == len(prefix_pages)
+        rows = [int(r) for m in members for r in m]
+        if len(set(rows)) != len(rows) or any(not 0 <= r < batch for r in rows):
+            raise ValueError(f"a batch row is in one group at most and below {batch}: {members}")
+        if any(p < 0 for p in prefix_pages):
+            raise ValueError(f"prefix_pages {prefix_pages}")
+        skip, start = [0] * batch, [0]
+        for m, p in zip(members, prefix_pages):
+            start.append(start[-1] + len(m))
+            for r in m:
+                skip[int(r)] = int(p)
+        self.batch, self.n_groups, self.max_members = batch, len(members), max((len(m) for m in members), default=0)
+        self.max_prefix = max(prefix_pages, default=0)
+        packed = torch.tensor(skip + start + rows, dtype=torch.int32).to(device)
+        self.skip, self.group_start, self.members = packed[:batch], packed[batch:batch + len(start)], packed[batch + len(start):]
+        pp = 128 // g.n_q_groups
+        ctas = g.h_kv * sum(-(-len(m) // pp) for m, p in zip(members, prefix_pages) if p)
+        self.n_split = n_split if n_split is not None else split_walk(max(1, ctas), max(1, self.max_prefix), device)
+
+
+def decode_shared_workspace(g: K2bGeom, batch: int, groups: PrefixGroups, device) -> torch.Tensor:
+    """Zero-initialised workspace for k2b_decode_shared (that of k2b_decode and the partial states of the prefixes)."""
+    n = int(_lib.lib().bmxk_k2b_decode_shared_workspace_bytes(ctypes.byref(g), batch, groups.n_split))
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int,
+                      groups: PrefixGroups, rope_cos: torch.Tensor, rope_sin: torch.Tensor, rope: torch.Tensor | None, k_tail: torch.Tensor | None,
+                      v_tail: torch.Tensor | None, tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor, sm_scale: float,
+                      workspace: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """k2b_decode for sequences that share prefixes (forks of a prompt): the prefix pages of a group are read and dequantized once for
+    all its members.  page_table rows are whole, prefix first; the members of a group have the same first pages there.  rope:
+    rope_fragments() of at least the longest prefix, or None (the tables are read as they are, slower).  Layout 1."""
+    g = pool.geom
+    assert q.dim() == 3 and groups.batch == q.shape[0], f"groups of a batch of {groups.batch}, queries of {q.shape[0]}"
+    with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, workspace,
+                       groups.skip):
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
+        rope_pages = _check_fragments(rope, groups.max_prefix)
+        out = _check_out(out, q, (torch.float16, torch.float32))
+        call("bmxk_k2b_decode_shared", ctypes.byref(g), _ptr(q), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16), _ptr(page_table),
+             page_table.stride(0), _ptr(n_pages), q.shape[0], max_pages, _ptr(groups.skip), _ptr(groups.members), _ptr(groups.group_start),
+             groups.n_groups, groups.max_members, groups.n_split, _ptr(rope_cos), _ptr(rope_sin), _ptr(rope), rope_pages, _ptr(k_tail), _ptr(v_tail),
+             _ptr(tail_len), tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), _ptr(workspace), workspace.numel(), _ptr(out),
+             _dtype_code(out), _stream())
+    return out
+
+
 def k2b_prefill_select(kernel: int) -> None:
     """Process-wide choice of the paged-prefill kernel: 0 = tcgen05 where it applies (default), 1 = mma.sync."""
     call("bmxk_k2b_prefill_select", int(kernel))
@@ -420,6 +608,55 @@ def window_shift(k_win: torch.Tensor, v_win: torch.Tensor, k_src_win: torch.Tens
     batch, h_kv, tail_cap = k_win.shape[0], k_win.shape[1], k_win.shape[2]
     call("bmxk_window_shift", _ptr(k_win), _ptr(v_win), _ptr(k_src_win), batch, h_kv, tail_cap, int(off), int(rest), _ptr(tail_len),
          _ptr(n_pages), int(pages_added), _stream())
+
+
+def _slot_list(slots) -> torch.Tensor:
+    t = slots if isinstance(slots, torch.Tensor) else torch.tensor(slots, dtype=None if len(slots) else torch.int64)
+    if t.is_cuda or t.dim() != 1 or t.is_floating_point() or t.dtype == torch.bool:
+        raise TypeError("copy_slots: slots are a list of integers or a 1-D integer tensor on the host")
+    if t.dtype != torch.int32:
+        if t.numel() and (int(t.min()) < -(1 << 31) or int(t.max()) >= 1 << 31):
+            raise ValueError("copy_slots: a slot does not fit 32 bits")
+        t = t.to(torch.int32)
+    return t.contiguous()
+
+
+def _slot_bytes(t: torch.Tensor) -> tuple[int, int]:
+    """(bytes of one slot, bytes from slot to slot) of an array whose first dimension counts slots."""
+    n = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and stride != n:
+            raise ValueError(f"copy_slots: the values of a slot must lie in one piece, strides {t.stride()} for shape {tuple(t.shape)}")
+        n *= size
+    item = t.element_size()
+    return n * item, (t.stride(0) if t.shape[0] > 1 else n) * item
+
+
+def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
+    """dsts[a][dst_slots[i]] = srcs[a][src_slots[i]] for all pairs i and arrays a, in one launch (per 3000 pairs).
+
+    The arrays (at most eight pairs of one shape behind dimension 0, e.g. pages and coefficients of a pool, or the rows of the three
+    windows, `k_win.flatten(0, 1)[:, :tail]`) have the slots in dimension 0; what a slot holds lies in one piece of a multiple of 16
+    bytes.  All sources have the same number of slots, and all destinations.  Slot lists are host integers.  A copy inside one array
+    must not write a slot that it reads, and no slot may be written twice: both are refused, like indices out of range."""
+    if len(srcs) != len(dsts) or not 1 <= len(srcs) <= 8:
+        raise ValueError(f"copy_slots: {len(srcs)} sources and {len(dsts)} destinations (1 to 8 of each)")
+    for s, d in zip(srcs, dsts):
+        if s.dtype != d.dtype or s.dim() < 2 or s.shape[1:] != d.shape[1:]:
+            raise ValueError(f"copy_slots: {tuple(s.shape)} {s.dtype} cannot be copied to {tuple(d.shape)} {d.dtype}")
+        if s.shape[0] != srcs[0].shape[0] or d.shape[0] != dsts[0].shape[0]:
+            raise ValueError("copy_slots: arrays of one call have the same number of slots")
+    a, b = _slot_list(src_slots), _slot_list(dst_slots)
+    if a.numel() != b.numel():
+        raise ValueError(f"copy_slots: {a.numel()} slots to read and {b.numel()} to write")
+    if a.numel() == 0:
+        return
+    n = len(srcs)
+    src_bytes, dst_bytes = [_slot_bytes(t) for t in srcs], [_slot_bytes(t) for t in dsts]
+    with _on_device_of(*srcs, *dsts):
+        call("bmxk_copy_slots", n, (ctypes.c_void_p * n)(*(t.data_ptr() for t in srcs)), (ctypes.c_void_p * n)(*(t.data_ptr() for t in dsts)),
+             (ctypes.c_int64 * n)(*(x[1] for x in src_bytes)), (ctypes.c_int64 * n)(*(x[1] for x in dst_bytes)),
+             (ctypes.c_int64 * n)(*(x[0] for x in src_bytes)), _ptr(a), _ptr(b), a.numel(), srcs[0].shape[0], dsts[0].shape[0], _stream())
 
 
 def step_ingest(q_src: torch.Tensor, q_dst: torch.Tensor, k_post: torch.Tensor, v: torch.Tensor, k_src: torch.Tensor,

@@ -20,31 +20,89 @@ HEAD_DIM = K.HEAD_DIM
 
 
 class PageAllocator:
-    """Free list over `n_slots` page slots (pure host code).  Slots of a sequence are returned in allocation order."""
+    """Free list over `n_slots` page slots (pure host code).  Slots of a sequence are returned in allocation order.  A slot may belong
+    to several sequences (share) and is free again when the last of them gives it back."""
 
     def __init__(self, n_slots: int):
         assert n_slots > 0
         self.n_slots = n_slots
         self._free = list(range(n_slots - 1, -1, -1))  # pop() hands out low slots first
         self._owned: dict[object, list[int]] = {}
+        self._refs: dict[int, int] = {}                # slot -> sequences that hold it
         self.peak_in_use = 0
 
-    def alloc(self, seq, n: int) -> list[int]:
-        """n more slots for sequence `seq`; raises MemoryError (and changes nothing) if the pool cannot hold them."""
+    def alloc(self, seq, n: int, places: list[int] | None = None, pages: int | None = None) -> list[int]:
+        """n more slots for sequence `seq`; raises MemoryError (and changes nothing) if the pool cannot hold them.  With places, the
+        sequence grows by `pages` pages of which only those at `places` (ascending, n of them) get a slot, the others -1."""
         if n > len(self._free):
             raise MemoryError(f"page pool exhausted: {n} slots wanted, {len(self._free)} of {self.n_slots} free")
         got = [self._free.pop() for _ in range(n)]
-        self._owned.setdefault(seq, []).extend(got)
+        for s in got:
+            self._refs[s] = 1
+        held = got
+        if places is not None:
+            held = [-1] * pages
+            for p, s in zip(places, got):
+                held[p] = s
+        self._owned.setdefault(seq, []).extend(held)
         self.peak_in_use = max(self.peak_in_use, self.in_use)
         return got
 
+    def _give_back(self, slots: list[int]) -> int:
+        """One holder less for each slot, in order; returns how many are free again."""
+        n = 0
+        for s in slots:
+            self._refs[s] -= 1
+            if self._refs[s] == 0:
+                del self._refs[s]
+                self._free.append(s)
+                n += 1
+        return n
+
     def free(self, seq) -> int:
-        """Returns every slot of `seq` to the free list; the count is returned."""
-        slots = self._owned.pop(seq, [])
-        self._free.extend(reversed(slots))
-        return len(slots)
+        """Gives back every slot of `seq`; returns how many of them nobody holds any more."""
+        return self._give_back([s for s in reversed(self._owned.pop(seq, [])) if s >= 0])
+
+    def share(self, seq, other) -> list[int]:
+        """`other`, which holds nothing yet, holds all slots of `seq` too (a fork: committed pages never change)."""
+        if self._owned.get(other):
+            raise ValueError(f"sequence {other!r} holds slots already")
+        slots = self._owned.get(seq, [])
+        for s in slots:
+            if s >= 0:
+                self._refs[s] += 1
+        self._owned[other] = list(slots)
+        return list(slots)
+
+    def release(self, seq, first: int, end: int) -> int:
+        """Gives back the slots of pages first .. end - 1 of `seq`, whose entries become -1 (pages that no query sees any more)."""
+        slots = self._owned.get(seq, [])
+        if not 0 <= first <= end <= len(slots):
+            raise ValueError(f"pages {first}..{end} of a sequence of {len(slots)}")
+        gone = [s for s in reversed(slots[first:end]) if s >= 0]
+        slots[first:end] = [-1] * (end - first)
+        return self._give_back(gone)
+
+    def available(self, seq, first: int, end: int) -> int:
+        """Slots that are free once release(seq, first, end) has been called."""
+        mine = self._owned.get(seq, [])[first:end]
+        return len(self._free) + sum(s >= 0 and self._refs[s] == 1 for s in mine)
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Renumbers the held slots to 0 .. in_use - 1 and returns the (from, to) lists of those that have to be copied: the ones
+        beyond, into the holes below, so that no slot is both read and written."""
+        m = self.in_use
+        holes = sorted(s for s in self._free if s < m)
+        moved = sorted(s for s in self._refs if s >= m)
+        new = dict(zip(moved, holes))
+        for slots in self._owned.values():
+            slots[:] = [new.get(s, s) for s in slots]
+        self._refs = {new.get(s, s): r for s, r in self._refs.items()}
+        self._free = list(range(self.n_slots - 1, m - 1, -1))
+        return moved, holes
 
     def slots(self, seq) -> list[int]:
+        """Slots of `seq` in page order; -1 for pages that were given back."""
         return list(self._owned.get(seq, ()))
 
     @property
@@ -56,6 +114,24 @@ class PageAllocator:
         self._free = list(range(self.n_slots + n_more - 1, self.n_slots - 1, -1)) + self._free
         self.n_slots += n_more
 
+    def shrink(self, n_slots: int) -> None:
+        """The pool behind this allocator was cut to its first n_slots slots, the others being free (see compact)."""
+        if any(s >= n_slots for s in self._refs):
+            raise ValueError(f"slots beyond {n_slots} are held")
+        self._free = [s for s in self._free if s < n_slots]
+        self.n_slots = n_slots
+
+
+def _runs(numbers: list[int]) -> list[tuple[int, int]]:
+    """Ascending integers -> their runs of consecutive ones as (begin, end)."""
+    out: list[tuple[int, int]] = []
+    for p in numbers:
+        if out and out[-1][1] == p:
+            out[-1] = (out[-1][0], p + 1)
+        else:
+            out.append((p, p + 1))
+    return out
+
 
 class PagedK2bLayer:
     """One attention layer's k2b cache for a changing set of sequences over one shared page pool.
@@ -63,10 +139,23 @@ class PagedK2bLayer:
     Each sequence has its own length, its own fp16 window row and its own run of page slots; all sequences share the frozen
     key basis of the layer (set with set_basis, or fitted on the first page that is ever committed).  `decode` runs one
     fused step over any subset of the live sequences.
+
+    `fork` makes sequences that share all committed pages of another one; a decode step that meets several sequences with a common
+    prefix reads it once for all of them.  With sliding_window, a token sees the last sliding_window tokens and the first `sinks`; pages
+    that fall between the two are freed as sequences grow.  `compact` and `resize` close the holes that finished sequences leave.
     """
 
+    # Pages of a shared prefix from which attending it once for `n` sequences beats streaming it n times (see _prefix_groups).
+    SHARED_MIN_ROWS = 12
+    SHARED_MIN_PAGES = 8
+
     def __init__(self, geom, n_slots: int, max_seqs: int, recent_window: int, device, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
-                 *, v_seed: int = 0, max_pages_per_seq: int = 1024):
+                 *, v_seed: int = 0, max_pages_per_seq: int = 1024, sliding_window: int | None = None, sinks: int = 0):
+        if sliding_window is not None and (sliding_window < 1 or sinks < 0 or geom.layout != 1):
+            raise ValueError(f"sliding_window={sliding_window}, sinks={sinks}: a window of at least one token over 128-token pages of layout 1")
+        if sliding_window is None and sinks:
+            raise ValueError("sinks without a sliding_window: every token is visible already")
+        self.sliding_window, self.sinks = sliding_window, sinks
         self.geom, self.device, self.page, self.W = geom, torch.device(device), geom.page, recent_window
         self.pool = K.K2bPool(geom, n_slots, self.device)
         self.alloc = PageAllocator(n_slots)
@@ -88,6 +177,8 @@ class PagedK2bLayer:
         self._committed: dict[object, int] = {}
         self._tail: dict[object, int] = {}
         self._ws: dict[int, torch.Tensor] = {}      # decode workspaces by batch size
+        self._groups: tuple | None = None           # the last step's page tables, its prefix groups and their workspace
+        self._rope_frag: torch.Tensor | None = None  # rotation tables in the prefill kernel's order, as far as prefixes reach
 
     # ---- bookkeeping ------------------------------------------------------------------------
     def set_basis(self, basis_f32: torch.Tensor) -> None:
@@ -109,6 +200,46 @@ class PagedK2bLayer:
     def seq_len(self, seq) -> int:
         return self._committed[seq] + self._tail[seq]
 
+    def fork(self, seq, *children) -> None:
+        """New sequences that begin with everything `seq` holds: its committed pages are shared (they never change, and are free again
+        when the last holder ends), its row of the fp16 windows is copied, in one launch for all children."""
+        row, t, h = self._rows[seq], self._tail[seq], self.geom.h_kv
+        if len(set(children)) != len(children) or any(c in self._rows for c in children):
+            raise ValueError(f"fork: {children} are live already or named twice")
+        if len(children) > len(self._free_rows):
+            raise MemoryError(f"{len(children)} sequence rows wanted, {len(self._free_rows)} of {self.max_seqs} free")
+        to = []
+        for c in children:
+            self.add_sequence(c)
+            self.alloc.share(seq, c)
+            self._committed[c], self._tail[c] = self._committed[seq], t
+            to += [self._rows[c] * h + i for i in range(h)]
+        if t and to:
+            wins = [w.flatten(0, 1)[:, :t] for w in (self.k_win, self.v_win, self.k_pre_win)]
+            K.copy_slots(wins, wins, [row * h + i for _ in children for i in range(h)], to)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest slots of the pool, in one launch; returns how many moved."""
+        moved, holes = self.alloc.compact()
+        K.copy_slots([self.pool.pages, self.pool.coefs], [self.pool.pages, self.pool.coefs], moved, holes)
+        return len(moved)
+
+    def resize(self, n_slots: int) -> None:
+        """A pool of n_slots slots takes this one's place, with the pages in use (MemoryError if they do not fit) in its lowest slots."""
+        m = self.alloc.in_use
+        if n_slots < max(1, m):
+            raise MemoryError(f"{m} slots are in use, {n_slots} wanted")
+        old, live = self.pool, sorted(self.alloc._refs)
+        pool = K.K2bPool(self.geom, n_slots, self.device)
+        moved, holes = self.alloc.compact()
+        now = dict(zip(moved, holes))
+        K.copy_slots([old.pages, old.coefs], [pool.pages, pool.coefs], live, [now.get(s, s) for s in live])
+        self.pool = pool
+        if n_slots > self.alloc.n_slots:
+            self.alloc.grow(n_slots - self.alloc.n_slots)
+        else:
+            self.alloc.shrink(n_slots)
+
     # ---- append -----------------------------------------------------------------------------
     def append(self, seq, k_pre: torch.Tensor, k_post: torch.Tensor, v: torch.Tensor) -> None:
         """n new tokens of one sequence, (h_kv, n, 128) each (fp16 or bf16): whole pages beyond the recent window are
@@ -120,14 +251,31 @@ class PagedK2bLayer:
         post = torch.cat([self.k_win[row, :, :t].to(k_post.dtype), k_post], 1) if t else k_post
         val = torch.cat([self.v_win[row, :, :t].to(v.dtype), v], 1) if t else v
         total = self._committed[seq] + t + n
+        p0 = self._committed[seq] // self.page
         n_flush = (compute_flush_schedule(total, self.W, self.page) - self._committed[seq]) // self.page
+        # sliding_window: the next query is the newest token or a later one, so the pages behind the sinks' and in front of the newest
+        # token's window are given back, and those among the new ones are never quantized
+        keep, first = p0 + n_flush, 0
+        if self.sliding_window is not None:
+            keep, first = -(-self.sinks // self.page), max(0, total - self.sliding_window) // self.page
+        kept = [p for p in range(p0, p0 + n_flush) if p < keep or p >= first]
+        old = self.alloc.slots(seq)
+        gone = (min(keep, p0), max(min(keep, p0), min(p0, first)))
+        if len(kept) > self.alloc.available(seq, *gone):
+            raise MemoryError(f"page pool exhausted: {len(kept)} slots wanted, {self.alloc.available(seq, *gone)} of {self.alloc.n_slots} free")
         if n_flush > 0:
+            assert len(old) + n_flush <= self.max_pages, "sequence longer than max_pages_per_seq pages"
             if self.basis_f32 is None:
                 self.set_basis(fit_basis(self.geom, src_k[:, : self.page]))
-            assert len(self.alloc.slots(seq)) + n_flush <= self.max_pages, "sequence longer than max_pages_per_seq pages"
-            slots = torch.tensor(self.alloc.alloc(seq, n_flush), dtype=torch.int32, device=self.device)
-            K.k2b_append(self.pool, src_k[None].contiguous(), val[None].to(src_k.dtype).contiguous(), self.basis_f32, self.signs,
-                         self.codebook, slots, n_flush)
+        self.alloc.release(seq, *gone)
+        if n_flush > 0:
+            got = dict(zip(kept, self.alloc.alloc(seq, len(kept), [p - p0 for p in kept], n_flush)))
+            k_all, v_all = src_k[None], val[None].to(src_k.dtype)
+            for a, b in _runs(kept):
+                slots = torch.tensor([got[p] for p in range(a, b)], dtype=torch.int32, device=self.device)
+                tok = slice((a - p0) * self.page, (b - p0) * self.page)
+                K.k2b_append(self.pool, k_all[:, :, tok].contiguous(), v_all[:, :, tok].contiguous(), self.basis_f32, self.signs, self.codebook,
+                             slots, b - a)
             self._committed[seq] += n_flush * self.page
         off = n_flush * self.page
         rest = post.shape[1] - off
@@ -136,25 +284,62 @@ class PagedK2bLayer:
         self._tail[seq] = rest
 
     # ---- decode -----------------------------------------------------------------------------
+    def _prefix_groups(self, slots: list) -> tuple[list, list]:
+        """(members, prefix pages) of the sequences that begin with the same slots.  A group is worth a pass of its own when it has
+        enough query rows per KV head (the prefix kernel's cost does not depend on them, the streaming kernel's grows with every
+        sequence) and enough pages."""
+        first: dict[int, list[int]] = {}
+        for i, s in enumerate(slots):
+            if s:
+                first.setdefault(s[0], []).append(i)
+        members, pages = [], []
+        for rows in first.values():
+            if len(rows) * self.geom.n_q_groups < self.SHARED_MIN_ROWS or len(rows) < 2:
+                continue
+            a, n = slots[rows[0]], min(len(slots[r]) for r in rows)
+            for r in rows[1:]:
+                s = slots[r]
+                if s[:n] != a[:n]:
+                    n = next(j for j in range(n) if s[j] != a[j])
+            if n >= self.SHARED_MIN_PAGES:
+                members.append(rows)
+                pages.append(n)
+        return members, pages
+
     def decode(self, seqs: list, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
-        """q (len(seqs), heads, 128) fp16: one fused decode step over those sequences, each with its own pages and window."""
+        """q (len(seqs), heads, 128) fp16: one fused decode step over those sequences, each with its own pages and window; a prefix
+        that several of them share is read once."""
         n = len(seqs)
         rows = torch.tensor([self._rows[s] for s in seqs], device=self.device)
-        max_pg = max(1, max(len(self.alloc.slots(s)) for s in seqs))
-        table = torch.zeros(n, max_pg, dtype=torch.int32)
-        for i, s in enumerate(seqs):
-            sl = self.alloc.slots(s)
-            table[i, : len(sl)] = torch.tensor(sl, dtype=torch.int32)
-        n_pages = torch.tensor([len(self.alloc.slots(s)) for s in seqs], dtype=torch.int32, device=self.device)
-        tail = torch.tensor([self._tail[s] for s in seqs], dtype=torch.int32, device=self.device)
-        if n not in self._ws:
-            self._ws[n] = K.decode_workspace(self.geom, n, max_pg, self.device)
-        any_pages = bool(int(n_pages.max()))
+        slots = [self.alloc.slots(s) for s in seqs]
+        counts = [len(s) for s in slots]
+        max_pg = max(1, max(counts))
+        table = torch.tensor([s + [0] * (max_pg - len(s)) for s in slots], dtype=torch.int32).to(self.device)
+        both = torch.tensor(counts + [self._tail[s] for s in seqs], dtype=torch.int32).to(self.device)
+        n_pages, tail = both[:n], both[n:]
+        max_walk = max_pg if any(counts) else 0
         basis16 = self.basis_f16 if self.basis_f16 is not None else torch.zeros(self.geom.h_kv * HEAD_DIM, self.geom.rank, dtype=torch.float16,
                                                                                  device=self.device)
-        return K.k2b_decode(self.pool, q, basis16, table.to(self.device), n_pages, max_pg if any_pages else 0, self.rope_cos, self.rope_sin,
-                            self.k_win[rows].contiguous(), self.v_win[rows].contiguous(), tail, self.v_lut, self.signs, self.sm_scale,
-                            self._ws[n], out=out)
+        tails = (self.k_win[rows].contiguous(), self.v_win[rows].contiguous(), tail)
+        last = (self.v_lut, self.signs, self.sm_scale)
+        if self.sliding_window is None and self.geom.layout == 1:
+            if self._groups is None or self._groups[0] != slots:
+                members, pages = self._prefix_groups(slots)
+                groups = K.PrefixGroups(self.geom, n, members, pages, self.device) if members else None
+                self._groups = (slots, groups, K.decode_shared_workspace(self.geom, n, groups, self.device) if groups else None)
+            _, groups, ws = self._groups
+            if groups is not None:
+                if self._rope_frag is None or self._rope_frag.shape[0] < groups.max_prefix:
+                    most = self.rope_cos.shape[0] // 128
+                    self._rope_frag = K.rope_fragments(self.rope_cos, self.rope_sin, min(most, 2 * groups.max_prefix))
+                return K.k2b_decode_shared(self.pool, q, basis16, table, n_pages, max_walk, groups, self.rope_cos, self.rope_sin, self._rope_frag,
+                                           *tails, *last, ws, out=out)
+        if n not in self._ws:
+            self._ws[n] = K.decode_workspace(self.geom, n, max_pg, self.device)
+        if self.sliding_window is not None:
+            return K.k2b_decode_sliding(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, self._ws[n],
+                                        self.sliding_window, self.sinks, out=out)
+        return K.k2b_decode(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, self._ws[n], out=out)
 
     # ---- accounting -------------------------------------------------------------------------
     def bytes_per_slot(self) -> int:

@@ -146,6 +146,34 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
                     size_t workspace_bytes, void* out, int out_dtype, float* partial_out, int phases,
                     void* stream);
 
+/* One decode step under a sliding window with sinks: of the keys a sequence holds, committed or in the fp16 window, the newest token (position
+ * total - 1, total = 128 * n_pages[s] + tail_len[s]) sees those at positions >= total - window (window >= 1: itself among them) and those
+ * < sinks.  Arguments as in bmxk_k2b_decode (no pos_offset, no partial states); layout 1 only.  Pages without a visible token are not
+ * read and their page-table entries may be anything: a caller frees them.  No per-step argument.  A sequence that holds nothing gives 0.
+ * (bmx's cache attends to everything it holds: src/bmx/cache/chunked_attention.py:398-530; a model's sliding layers have no path there.) */
+int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                            const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const void* rope_cos,
+                            const void* rope_sin, const void* k_tail, const void* v_tail, const int32_t* tail_len, int tail_cap,
+                            const uint32_t* v_lut, const float* signs, float sm_scale, int64_t window, int64_t sinks, void* workspace,
+                            size_t workspace_bytes, void* out, int out_dtype, void* stream);
+
+/* One decode step for sequences that share prefixes of whole pages: group z is the sequences members[group_start[z]] ..
+ * members[group_start[z + 1] - 1] (each sequence in one group at most), whose page-table rows begin with the same skip[s] entries
+ * (skip[s] = 0 for a sequence in no group).  A group's prefix is dequantized once for 128 / n_q_groups sequences at a time and its
+ * pages are shared out over n_split CTAs; the pages behind it, the fp16 window and the merge are those of bmxk_k2b_decode, whose
+ * arguments and result these are (no pos_offset, no partial states).  skip, members, group_start: int32 device arrays; max_members: the
+ * largest group.  rope_frag: bmxk_k2b_rope_fragments of rope_pages pages (every prefix has to lie within, see the status word (3,
+ * rope_pages, pages)), or null: the tables are read as they are, about a quarter slower.  Layout 1, sm_scale > 0.  workspace:
+ * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once.  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every
+ * sequence has a cache of its own.) */
+size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split);
+int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
+                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
+                           const int32_t* members, const int32_t* group_start, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
+                           const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
+                           size_t workspace_bytes, void* out, int out_dtype, void* stream);
+
 /* Causal attention of n_q new query positions per sequence over the committed pages and the fp16 window, without
  * building dense K / V for the context: each 128-token page is dequantized into shared memory and attended there.
  * bmx: src/bmx/cache/chunked_attention.py:320-395 _prefill_dense_attention (dequantize every page, then SDPA with the
@@ -184,6 +212,21 @@ int bmxk_k2b_prefill_rope(const bmxk_k2b_geom* g, const void* q, int n_q, int64_
                           const void* rope_cos, const void* rope_sin, int64_t pos_offset, const void* k_tail, const void* v_tail,
                           const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale,
                           int32_t* status, void* out, int n_split, int rope_pages, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The rotation tables of positions 0 .. 128 * n_pages - 1 in the order in which the key warps of the prefill kernel read them, for callers
+ * that attend often and keep them: frag has bmxk_k2b_prefill_rope_bytes(n_pages) bytes, everything 16-byte aligned. */
+int bmxk_k2b_rope_fragments(const void* rope_cos, const void* rope_sin, int n_pages, void* frag, void* stream);
+
+/* bmxk_k2b_prefill_split under a sliding window with sinks: query row i at position x = q_pos0 + i sees the keys at positions in (x - window, x]
+ * and those < min(sinks, x + 1).  Pages that no row sees are not read and their page-table entries may be anything.  rope_frag: see
+ * bmxk_k2b_rope_fragments (every page that a row's position reaches has to lie within rope_pages), or null.  q and out 16-byte
+ * aligned, sm_scale > 0.  A row that sees nothing gives 0. */
+int bmxk_k2b_prefill_sliding(const bmxk_k2b_geom* g, const void* q, int n_q, int64_t q_pos0, const void* pages, const void* coefs,
+                             const void* basis_f16, const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch,
+                             const void* rope_cos, const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail,
+                             const void* v_tail, const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale,
+                             int64_t window, int64_t sinks, int32_t* status, void* out, int n_split, void* workspace, size_t workspace_bytes,
+                             void* stream);
 
 /* Which kernel bmxk_k2b_prefill launches (process-wide; no counterpart in bmx).  0 (default): the tcgen05 kernel when q
  * and out are 16-byte aligned and sm_scale is positive, else the mma.sync kernel; 1: always the mma.sync kernel.  Both give the same attention
@@ -414,6 +457,18 @@ int bmxk_window_shift(void* k_win, void* v_win, void* k_src_win, int batch, int 
  * these slots, windows shifted, decode -- has no per-step argument and replays as a CUDA graph like any other step. */
 int bmxk_gather_next_slots(const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int n,
                            int32_t* slots_out, void* stream);
+
+/* ---- slots of a pool ---------------------------------------------------------------------- */
+/* dst[a][dst_slots[i]] = src[a][src_slots[i]] for every pair i < n and array a < n_arrays (1..8), one launch per 3000 pairs (no
+ * counterpart in bmx, whose pages are Python dicts: forking a sequence, closing the holes of a pool, taking a pool over into another).
+ * Slot i of an array begins i * stride bytes behind its base and `bytes` of it are copied (a row of a window may be copied in part).
+ * src, dst, src_stride, dst_stride, bytes and the two slot lists are HOST arrays, read before the call returns; the copies themselves run
+ * in stream order and the launch can be captured.  Bases, strides and sizes are multiples of 16 bytes.  Refused: a slot outside
+ * [0, n_src_slots) / [0, n_dst_slots), a slot written twice, and, where a destination IS a source (a copy inside one pool), a slot
+ * both read and written; arrays that overlap in any other way. */
+int bmxk_copy_slots(int n_arrays, const void* const* src, void* const* dst, const int64_t* src_stride, const int64_t* dst_stride,
+                    const int64_t* bytes, const int32_t* src_slots, const int32_t* dst_slots, int n, int64_t n_src_slots, int64_t n_dst_slots,
+                    void* stream);
 
 /* A decode step's inputs in one launch (no counterpart in bmx, whose step starts from device tensors): the append of
  * bmxk_window_append_devpos for fp16 sources, plus the step's queries q_src (batch, h_kv*n_q_groups, 128) fp16 staged
