@@ -138,8 +138,7 @@ _SIGNATURES = {
     "bmxk_k2b_decode_shared": (c_int, [POINTER(K2bGeom), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
                                        c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                        c_int, c_void_p, c_void_p, c_float, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
-    "bmxk_copy_slots": (c_int, [c_int, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_void_p,
-                                c_void_p, c_int, c_int64, c_int64, c_void_p]),
+    "bmxk_copy_slots": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),
     "bmxk_check_workspace_status": (c_int, [c_void_p, c_void_p]),
     "bmxk_k2b_decode_static_status": (c_int, [c_void_p]),
     "bmxk_selftest_bounded_wait": (c_int, [c_void_p, ctypes.c_int64, c_void_p]),

@@ -61,6 +61,7 @@ struct TileCursor {
 constexpr int WALK_ALL = 0, WALK_OWN = 1, WALK_SLIDING = 2;
 struct K2bWalk {
   const int32_t* skip;
+  bool after_prefix;  // WALK_OWN: the prefix kernel was launched just before on the same stream; see launch_decode_t5
   const int32_t* tail_len;  // WALK_SLIDING: tokens in the fp16 window, or null
   int tail_cap;
   int64_t window;
@@ -179,7 +180,10 @@ int num_sms();
 // kernel is then launched as its programmatic dependent: its blocks may start while that kernel drains, attend over
 // the fp16 window (which that kernel does not write) and wait for it only before they read the partial states.
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = false, int walk = WALK_ALL);
-// tcgen05 decode kernel for layout-1 pools (k2b_decode_t5.cu); two partial records per slot (one per tile parity)
+// tcgen05 decode kernel for layout-1 pools (k2b_decode_t5.cu); two partial records per slot (one per tile parity).  Behind a prefix kernel
+// (walk.after_prefix) it is launched as that kernel's programmatic dependent: its blocks take over SMs as the prefix blocks finish (it reads
+// nothing of theirs), and each waits for the prefix kernel's completion before it ends, so that the merge kernel, which waits for this
+// one, finds both kernels' records.
 int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk = WALK_ALL);
 
 }  // namespace bmxk

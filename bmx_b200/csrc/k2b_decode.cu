@@ -419,8 +419,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) k2b_decode_kernel(const K2bDec
 // and one after it (all partial records of a thread in flight together).
 // ---------------------------------------------------------------------------------------------
 constexpr int MERGE_THREADS = 256;
+constexpr size_t GROUP_MERGE_SMEM = 200 * 1024;
 
-template <int WALK>
 __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMergeParams p) {
   extern __shared__ __align__(16) float msm[];
   const K2bGeom g = p.g;
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   if (warp == 0) {
     int pre = 0, tot = 0;
     for (int i = lane; i < p.batch; i += 32) {
-      const int t = (WALK == WALK_ALL ? tiles_of(p.n_pages[i], g.page) : page_span<WALK>(p.walk, p.n_pages[i], i).tiles) * g.h_kv;
+      const int t = tiles_of(p.n_pages[i], g.page) * g.h_kv;
       tot += t;
       if (i < b) pre += t;
     }
@@ -453,14 +453,6 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   const int tl = p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
   const __half* kt = p.k_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
   const __half* vt = p.v_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
-  // WALK_SLIDING: window tokens [hid0, hid1) lie behind the sinks and in front of the sliding window: left out
-  int hid0 = 0, hid1 = 0;
-  if constexpr (WALK == WALK_SLIDING) {
-    const int64_t tail0 = (int64_t)p.n_pages[b] * TILE_TOKENS;
-    hid0 = (int)max((int64_t)0, min((int64_t)tl, p.walk.sinks - tail0));
-    hid1 = max(hid0, (int)max((int64_t)0, tl - p.walk.window));
-  }
-  auto shown = [&](int t) { return t < tl && (WALK != WALK_SLIDING || t < hid0 || t >= hid1); };
   float mx = -INFINITY;
   {
     const int l8 = tid & 7, tp = tid >> 3;
@@ -488,11 +480,9 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
         d += __shfl_xor_sync(0xffffffffu, d, 1);
         d += __shfl_xor_sync(0xffffffffu, d, 2);
         d += __shfl_xor_sync(0xffffffffu, d, 4);
-        if (shown(t)) {
+        if (t < tl) {
           mx = fmaxf(mx, d);
           if (l8 == 0) sc[t] = d;
-        } else if (WALK == WALK_SLIDING && t < tl && l8 == 0) {
-          sc[t] = -INFINITY;
         }
       }
     }
@@ -504,7 +494,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int t = tg + 16 * i;
-    vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
+    vv[i] = (t < tl) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
@@ -534,7 +524,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = t0 + tg + 16 * i;
-          vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
+          vv[i] = (t < tl) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
         }
       }
 #pragma unroll
@@ -569,7 +559,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
   //      CTA cta0 + r % n_cta.  Thread = (record parity, channel): an online softmax over its records ----
   const int total = si[1];
   const int per_cta = max(1, (total + p.main_grid - 1) / p.main_grid);
-  const int tiles_b = (WALK == WALK_ALL) ? tiles_of(p.n_pages[b], g.page) : page_span<WALK>(p.walk, p.n_pages[b], b).tiles;
+  const int tiles_b = tiles_of(p.n_pages[b], g.page);
   const int T0 = si[0] + h * tiles_b, T1 = T0 + tiles_b;
   const int cta0 = T0 / per_cta, cta1 = (tiles_b > 0) ? (T1 - 1) / per_cta : cta0 - 1;
   const int sub_slots = p.main_grid + p.batch * g.h_kv;
@@ -601,28 +591,6 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
         L = L * fo + l_[j] * fn, A = A * fo + a_[j] * fn, M = Mn;
       }
     }
-    if constexpr (WALK == WALK_OWN) {
-      // the shared prefix's records of this row (same units: the value rotation is undone below, once for both)
-      const float* pr = p.prefix_part + ((int64_t)bh * G + qi) * p.prefix_split * PREFIX_PART_STRIDE;
-      const int n_pre = p.walk.skip[b] > 0 ? p.prefix_split : 0;
-      for (int r0 = half; r0 < n_pre; r0 += 8) {
-        float m_[4], l_[4], a_[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = r0 + 2 * j;
-          const float* ps = pr + (int64_t)r * PREFIX_PART_STRIDE;
-          if (r < n_pre) m_[j] = ps[128], l_[j] = ps[129], a_[j] = ps[ch];
-          else m_[j] = -INFINITY, l_[j] = 0.f, a_[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float Mn = fmaxf(M, m_[j]);
-          const float fo = (M == -INFINITY) ? 0.f : ex2_approx(M - Mn);
-          const float fn = (m_[j] == -INFINITY) ? 0.f : ex2_approx(m_[j] - Mn);
-          L = L * fo + l_[j] * fn, A = A * fo + a_[j] * fn, M = Mn;
-        }
-      }
-    }
     red[half * HEAD_DIM + ch] = A;
     if (ch == 0) sm[16 + 2 * half] = M, sm[17 + 2 * half] = L;
   }
@@ -640,12 +608,10 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = x[k] * p.signs[4 * lane + k] * 0.08838834764831845f;
     }
-    // Nothing to attend to (an empty sequence): 0 in the walks that came with shared prefixes and sliding windows
     const float mw = (tl > 0) ? m_w : -INFINITY;
     const float Mf = fmaxf(Mp, mw);
     const float fp = (Mp == -INFINITY) ? 0.f : ex2_approx(Mp - Mf), fw = (mw == -INFINITY) ? 0.f : ex2_approx(mw - Mf);
-    float l = Lp * fp + ((tl > 0) ? l_w : 0.f) * fw;
-    if (WALK != WALK_ALL && l == 0.f) l = 1.f;
+    const float l = Lp * fp + ((tl > 0) ? l_w : 0.f) * fw;
     const int64_t row = (int64_t)bh * G + qi;
     float val[4];
 #pragma unroll
@@ -662,6 +628,247 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
       const __half2 h01 = __floats2half2_rn(val[0] / l, val[1] / l), h23 = __floats2half2_rn(val[2] / l, val[3] / l);
       *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + row * HEAD_DIM + 4 * lane) = make_uint2(h2_as_u32(h01), h2_as_u32(h23));
     }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Merge of a step under a sliding window or behind shared prefixes: one block of 256 threads per (sequence, KV head) serves all its query
+// heads, so that a window row is read and widened once for the group (the kernel above reads it once per query head).  Against a variant
+// of that kernel, in a step of 128 sequences x 8 KV heads x 4 query heads with 4 prefix records each: 87 -> 35 us; 32 sequences with 18
+// records 26 -> 10 us; one sequence: the same time.
+//   scores   2 * GQ lanes per token, 64 / GQ channels each (64 query values per lane in registers); the GQ partial sums are reduced by
+//            halves: each step a lane keeps the sums of half of its queries and hands over the other half
+//   values   thread = (channel octet, token group of 16), GQ x 8 accumulators; every row is loaded once
+//   records  warp = query head (and half of the records for GQ = 4), lane = four channels, all loads of four records in flight
+// ---------------------------------------------------------------------------------------------
+template <int WALK, int GQ>
+__global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_group_kernel(const K2bMergeParams p) {
+  constexpr int LPT = 2 * GQ, CH = 64 / GQ, TPP = MERGE_THREADS / LPT;  // lanes per token, channels per lane, tokens per pass
+  constexpr int NB = 4;                                                // passes whose loads are in flight together
+  extern __shared__ __align__(16) float msm[];
+  const K2bGeom g = p.g;
+  const int G = g.n_q_groups, cap4 = (p.tail_cap + 3) & ~3;
+  float* sc = msm;                    // [GQ][cap4] window scores, then weights
+  float* red = sc + GQ * cap4;        // [8][GQ][128] window accumulators per warp
+  float* qs = red;                    // [GQ][128] scaled queries, before that
+  float* rec = red + 8 * GQ * HEAD_DIM;  // [4][32][4] accumulators of the second half of the records (GQ = 4)
+  float* sm = rec + 4 * HEAD_DIM;        // [8] window maxima, [8] window sums, [4][2] states of the second half
+  int* si = reinterpret_cast<int*>(sm + 24);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bh = blockIdx.x, b = bh / g.h_kv, h = bh % g.h_kv;
+
+  if (warp == 0) {
+    int pre = 0, tot = 0;
+    for (int i = lane; i < p.batch; i += 32) {
+      const int t = page_span<WALK>(p.walk, p.n_pages[i], i).tiles * g.h_kv;
+      tot += t;
+      if (i < b) pre += t;
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) pre += __shfl_xor_sync(0xffffffffu, pre, m), tot += __shfl_xor_sync(0xffffffffu, tot, m);
+    if (lane == 0) si[0] = pre, si[1] = tot;
+  }
+  for (int i = tid; i < GQ * HEAD_DIM; i += MERGE_THREADS)
+    qs[i] = i < G * HEAD_DIM ? __half2float(p.q[(int64_t)bh * G * HEAD_DIM + i]) * p.scale_log2 : 0.f;
+  __syncthreads();
+
+  const int tl = p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
+  const __half* kt = p.k_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
+  const __half* vt = p.v_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
+  int hid0 = 0, hid1 = 0;
+  if constexpr (WALK == WALK_SLIDING) {
+    const int64_t tail0 = (int64_t)p.n_pages[b] * TILE_TOKENS;
+    hid0 = (int)max((int64_t)0, min((int64_t)tl, p.walk.sinks - tail0));
+    hid1 = max(hid0, (int)max((int64_t)0, tl - p.walk.window));
+  }
+  auto shown = [&](int t) { return t < tl && (WALK != WALK_SLIDING || t < hid0 || t >= hid1); };
+  {
+    const int l = tid % LPT, tp = tid / LPT;
+    float qr[GQ][CH];
+#pragma unroll
+    for (int qi = 0; qi < GQ; ++qi)
+#pragma unroll
+      for (int k = 0; k < CH; ++k) qr[qi][k] = qs[qi * HEAD_DIM + 64 * (k / 8) + 8 * l + k % 8];  // chunks l and, with 16 channels, 8 + l
+    for (int t0 = 0; t0 < tl; t0 += NB * TPP) {
+      uint4 kv[NB][CH / 8];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int t = t0 + i * TPP + tp;
+#pragma unroll
+        for (int c = 0; c < CH / 8; ++c)
+          kv[i][c] = shown(t) ? reinterpret_cast<const uint4*>(kt + (int64_t)t * HEAD_DIM)[l + 8 * c] : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        float d[GQ];
+#pragma unroll
+        for (int qi = 0; qi < GQ; ++qi) d[qi] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH / 8; ++c) {
+          const uint32_t w[4] = {kv[i][c].x, kv[i][c].y, kv[i][c].z, kv[i][c].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(u32_as_h2(w[k]));
+#pragma unroll
+            for (int qi = 0; qi < GQ; ++qi) d[qi] = fmaf(f.y, qr[qi][8 * c + 2 * k + 1], fmaf(f.x, qr[qi][8 * c + 2 * k], d[qi]));
+          }
+        }
+#pragma unroll
+        for (int m = GQ / 2; m >= 1; m >>= 1) {
+          const bool up = (l & m) != 0;
+#pragma unroll
+          for (int k = 0; k < m; ++k) {
+            const float mine = up ? d[m + k] : d[k], other = up ? d[k] : d[m + k];
+            d[k] = mine + __shfl_xor_sync(0xffffffffu, other, m);
+          }
+        }
+        d[0] += __shfl_xor_sync(0xffffffffu, d[0], GQ);
+        const int t = t0 + i * TPP + tp;
+        if (l < GQ && t < tl) sc[l * cap4 + t] = shown(t) ? d[0] : -INFINITY;  // lane l ends with query l
+      }
+    }
+  }
+  // ---- values: the first rows travel during the softmax ----
+  const int c8 = tid & 15, tg = tid >> 4;
+  uint4 vv[NB];
+  auto load_values = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int t = t0 + tg + 16 * i;
+      vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  load_values(0);
+  __syncthreads();
+  if (warp < GQ) {
+    float mx = -INFINITY, ls = 0.f;
+    for (int t = lane; t < tl; t += 32) mx = fmaxf(mx, sc[warp * cap4 + t]);
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+    for (int t = lane; t < tl; t += 32) {
+      const float e = ex2_approx(sc[warp * cap4 + t] - mx);
+      sc[warp * cap4 + t] = e, ls += e;
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, m);
+    if (lane == 0) sm[warp] = mx, sm[8 + warp] = ls;
+  }
+  __syncthreads();
+  {
+    float a[GQ][8];
+#pragma unroll
+    for (int qi = 0; qi < GQ; ++qi)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[qi][k] = 0.f;
+    for (int t0 = 0; t0 < tl; t0 += 16 * NB) {
+      if (t0 > 0) load_values(t0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int t = t0 + tg + 16 * i;
+        const uint32_t w[4] = {vv[i].x, vv[i].y, vv[i].z, vv[i].w};
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = __half22float2(u32_as_h2(w[k]));
+          f[2 * k] = x.x, f[2 * k + 1] = x.y;
+        }
+#pragma unroll
+        for (int qi = 0; qi < GQ; ++qi) {
+          const float wgt = (t < tl) ? sc[qi * cap4 + t] : 0.f;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) a[qi][k] = fmaf(wgt, f[k], a[qi][k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int qi = 0; qi < GQ; ++qi) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[qi][k] += __shfl_xor_sync(0xffffffffu, a[qi][k], 16);
+      if (lane < 16) {
+        float4* o = reinterpret_cast<float4*>(red + (warp * GQ + qi) * HEAD_DIM + 8 * c8);
+        o[0] = make_float4(a[qi][0], a[qi][1], a[qi][2], a[qi][3]), o[1] = make_float4(a[qi][4], a[qi][5], a[qi][6], a[qi][7]);
+      }
+    }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // as in the kernel above
+  __syncthreads();
+
+  const int per_cta = max(1, (si[1] + p.main_grid - 1) / p.main_grid);
+  const int tiles_b = page_span<WALK>(p.walk, p.n_pages[b], b).tiles;
+  const int T0 = si[0] + h * tiles_b, T1 = T0 + tiles_b;
+  const int cta0 = T0 / per_cta, cta1 = (tiles_b > 0) ? (T1 - 1) / per_cta : cta0 - 1;
+  const int sub_slots = p.main_grid + p.batch * g.h_kv;
+  const int n_cta = max(0, cta1 - cta0 + 1), n_own = n_cta * p.n_sub;
+  const int n_pre = (WALK == WALK_OWN && p.walk.skip[b] > 0) ? p.prefix_split : 0;
+  constexpr int PARTS = 8 / GQ;  // warps per query head
+  const int qi = warp % GQ, part = warp / GQ;
+  float M = -INFINITY, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+  if (qi < G) {
+    const float* pre = p.prefix_part + ((int64_t)bh * G + qi) * p.prefix_split * PREFIX_PART_STRIDE;
+    for (int r0 = part; r0 < n_own + n_pre; r0 += NB * PARTS) {
+      float m_[NB], l_[NB];
+      float2 a_[NB][2];
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int r = r0 + j * PARTS;
+        m_[j] = -INFINITY, l_[j] = 0.f, a_[j][0] = a_[j][1] = make_float2(0.f, 0.f);
+        if (r < n_own) {
+          const int sb = r / n_cta, c = cta0 + (r - sb * n_cta);
+          const float* ps = p.part + ((int64_t)(sb * sub_slots + c + bh) * G + qi) * PART_STRIDE;
+          m_[j] = ps[0], l_[j] = ps[1];
+          a_[j][0] = reinterpret_cast<const float2*>(ps + 2)[2 * lane], a_[j][1] = reinterpret_cast<const float2*>(ps + 2)[2 * lane + 1];
+        } else if (WALK == WALK_OWN && r < n_own + n_pre) {
+          const float* ps = pre + (int64_t)(r - n_own) * PREFIX_PART_STRIDE;
+          const float4 x = reinterpret_cast<const float4*>(ps)[lane];
+          m_[j] = ps[128], l_[j] = ps[129], a_[j][0] = make_float2(x.x, x.y), a_[j][1] = make_float2(x.z, x.w);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const float Mn = fmaxf(M, m_[j]);
+        const float fo = (M == -INFINITY) ? 0.f : ex2_approx(M - Mn);
+        const float fn = (m_[j] == -INFINITY) ? 0.f : ex2_approx(m_[j] - Mn);
+        L = L * fo + l_[j] * fn, M = Mn;
+        A[0] = A[0] * fo + a_[j][0].x * fn, A[1] = A[1] * fo + a_[j][0].y * fn;
+        A[2] = A[2] * fo + a_[j][1].x * fn, A[3] = A[3] * fo + a_[j][1].y * fn;
+      }
+    }
+  }
+  if constexpr (PARTS == 2) {
+    if (part == 1) {
+      reinterpret_cast<float4*>(rec)[qi * 32 + lane] = make_float4(A[0], A[1], A[2], A[3]);
+      if (lane == 0) sm[16 + 2 * qi] = M, sm[17 + 2 * qi] = L;
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float M1 = sm[16 + 2 * qi], L1 = sm[17 + 2 * qi], Mp = fmaxf(M, M1);
+    const float f0 = (M == -INFINITY) ? 0.f : ex2_approx(M - Mp), f1 = (M1 == -INFINITY) ? 0.f : ex2_approx(M1 - Mp);
+    const float4 x = reinterpret_cast<const float4*>(rec)[qi * 32 + lane];
+    A[0] = A[0] * f0 + x.x * f1, A[1] = A[1] * f0 + x.y * f1, A[2] = A[2] * f0 + x.z * f1, A[3] = A[3] * f0 + x.w * f1;
+    L = L * f0 + L1 * f1, M = Mp;
+  }
+  if (qi >= G) return;
+  fwht128_warp(A, lane);
+  float win[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float4 x = reinterpret_cast<const float4*>(red + (w * GQ + qi) * HEAD_DIM)[lane];
+    win[0] += x.x, win[1] += x.y, win[2] += x.z, win[3] += x.w;
+  }
+  const float mw = (tl > 0) ? sm[qi] : -INFINITY, lw = (tl > 0) ? sm[8 + qi] : 0.f;
+  const float Mf = fmaxf(M, mw);
+  const float fp = (M == -INFINITY) ? 0.f : ex2_approx(M - Mf), fw = (mw == -INFINITY) ? 0.f : ex2_approx(mw - Mf);
+  float l = L * fp + lw * fw;
+  if (l == 0.f) l = 1.f;  // nothing to attend to: 0
+  float val[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) val[k] = (A[k] * p.signs[4 * lane + k] * 0.08838834764831845f) * fp + win[k] * fw;
+  const int64_t row = (int64_t)bh * G + qi;
+  if (p.out_dtype == BMXK_DTYPE_F32) {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + row * HEAD_DIM + 4 * lane) = make_float4(val[0] / l, val[1] / l, val[2] / l, val[3] / l);
+  } else {
+    const __half2 h01 = __floats2half2_rn(val[0] / l, val[1] / l), h23 = __floats2half2_rn(val[2] / l, val[3] / l);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + row * HEAD_DIM + 4 * lane) = make_uint2(h2_as_u32(h01), h2_as_u32(h23));
   }
 }
 
@@ -709,24 +916,48 @@ int num_sms() {
   return n;
 }
 
-int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
-  const int G = mp.g.n_q_groups;
-  const size_t msmem = ((size_t)((mp.tail_cap + 3) & ~3) + (1 + 16 + 1) * HEAD_DIM + 32 + 4) * sizeof(float);
-  BMXK_REQUIRE(msmem <= 48 * 1024, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
+template <class Kernel>
+static int launch_merge_kernel(Kernel kernel, const K2bMergeParams& mp, unsigned grid, size_t smem, cudaStream_t s, bool after_main) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(mp.batch * mp.g.h_kv * G)), cfg.blockDim = dim3(MERGE_THREADS), cfg.dynamicSmemBytes = msmem, cfg.stream = s;
+  cfg.gridDim = dim3(grid), cfg.blockDim = dim3(MERGE_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = after_main ? 1 : 0;
-  const cudaError_t e = walk == WALK_OWN       ? cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_OWN>, mp)
-                        : walk == WALK_SLIDING ? cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_SLIDING>, mp)
-                                               : cudaLaunchKernelEx(&cfg, k2b_merge_kernel<WALK_ALL>, mp);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mp);
   if (e != cudaSuccess) {
     set_error("decode(merge): %s", cudaGetErrorString(e));
     return BMXK_ERR_CUDA;
   }
   return check_launch("decode(merge)");
+}
+
+template <int WALK, int GQ>
+static int launch_merge_group(const K2bMergeParams& mp, size_t smem, cudaStream_t s, bool after_main) {
+  static PerDeviceOnce configured;
+  if (configured.first()) {
+    const cudaError_t e = cudaFuncSetAttribute(k2b_merge_group_kernel<WALK, GQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, GROUP_MERGE_SMEM);
+    if (e != cudaSuccess) {
+      configured.retract();
+      set_error("decode(merge): cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      return BMXK_ERR_CUDA;
+    }
+  }
+  return launch_merge_kernel(k2b_merge_group_kernel<WALK, GQ>, mp, (unsigned)(mp.batch * mp.g.h_kv), smem, s, after_main);
+}
+
+int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
+  const int G = mp.g.n_q_groups, gq = G <= 4 ? 4 : 8;
+  if (walk != WALK_ALL) {
+    const size_t gsmem = ((size_t)gq * ((mp.tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
+    BMXK_REQUIRE(gsmem <= GROUP_MERGE_SMEM, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
+    if (walk == WALK_OWN) return gq == 4 ? launch_merge_group<WALK_OWN, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_OWN, 8>(mp, gsmem, s, after_main);
+    return gq == 4 ? launch_merge_group<WALK_SLIDING, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_SLIDING, 8>(mp, gsmem, s, after_main);
+  }
+  const size_t msmem = ((size_t)((mp.tail_cap + 3) & ~3) + (1 + 16 + 1) * HEAD_DIM + 32 + 4) * sizeof(float);
+  BMXK_REQUIRE(msmem <= 48 * 1024, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
+  const unsigned grid = (unsigned)(mp.batch * mp.g.h_kv * G);
+  return launch_merge_kernel(k2b_merge_kernel, mp, grid, msmem, s, after_main);
 }
 
 static size_t decode_stage_bytes(const bmxk_k2b_geom* g) {
@@ -906,7 +1137,7 @@ size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch,
 
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
                            const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
-                           const int32_t* members, const int32_t* group_start, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
                            const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
                            const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
                            size_t workspace_bytes, void* out, int out_dtype, void* stream) {
@@ -919,7 +1150,7 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   BMXK_REQUIRE(batch >= 1 && max_pages >= 0 && n_groups >= 0 && n_groups <= 65535 && max_members >= 0 && max_members <= batch,
                "bmxk_k2b_decode_shared: batch=%d max_pages=%d n_groups=%d max_members=%d", batch, max_pages, n_groups, max_members);
   BMXK_REQUIRE(n_split >= 1 && n_split <= 64, "bmxk_k2b_decode_shared: n_split=%d must be in 1..64", n_split);
-  BMXK_REQUIRE(skip && (n_groups == 0 || (members && group_start)), "bmxk_k2b_decode_shared: null group lists");
+  BMXK_REQUIRE(skip && (n_groups == 0 || (members && groups && ((uintptr_t)groups & 15) == 0)), "bmxk_k2b_decode_shared: null or misaligned group lists");
   BMXK_REQUIRE(sm_scale > 0.f, "bmxk_k2b_decode_shared: sm_scale=%g must be positive", sm_scale);
   BMXK_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= bmxk_k2b_decode_shared_workspace_bytes(g, batch, n_split),
                "bmxk_k2b_decode_shared: workspace of %zu bytes needed (16-byte aligned), %zu given",
@@ -945,13 +1176,13 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
     memcpy(&prm.lut_alpha, &v_lut[2], 4);
     memcpy(&prm.lut_beta, &v_lut[3], 4);
     prm.signs = signs, prm.scale_log2 = sm_scale * 1.4426950408889634f, prm.status = (int32_t*)workspace;
-    prm.n_split = n_split, prm.part = part, prm.skip = skip, prm.members = members, prm.group_start = group_start;
+    prm.n_split = n_split, prm.part = part, prm.members = members, prm.groups = groups;
     const int pp = 128 / g->n_q_groups;
     const int rc = launch_prefix_t5(prm, dim3((unsigned)((max_members + pp - 1) / pp * n_split), (unsigned)g->h_kv, (unsigned)n_groups), (cudaStream_t)stream);
     if (rc) return rc;
   }
   K2bWalk w = {};
-  w.skip = skip;
+  w.skip = skip, w.after_prefix = prefixes;
   return decode_step(g, q, pages, coefs, basis_f16, page_table, table_stride, n_pages, batch, max_pages, rope_cos, rope_sin, 0, k_tail, v_tail,
                      tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, nullptr, 3, WALK_OWN, w, max_pages,
                      part, n_split, stream);

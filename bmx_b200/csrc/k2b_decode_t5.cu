@@ -132,7 +132,22 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   const int f_begin = min(total, (int)blockIdx.x * per_cta);
   const int f_end = min(total, f_begin + per_cta);
   const int n_tiles = f_end - f_begin;
-  if (n_tiles <= 0) return;
+  if (n_tiles <= 0) {
+    if constexpr (WALK == WALK_OWN) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+
+  Walker w;
+  w.init(cum, npg_sm, f_begin, g.h_kv);
+  // The basis operand of the first range.  Where every page is streamed the rotation warp lays it out with the range's first tile (a CTA
+  // walks a hundred tiles); the other walks are short, and one warp's 16 dependent loads would be a third of the time to the first product.
+  if constexpr (WALK != WALK_ALL) {
+    const uint4* bs = reinterpret_cast<const uint4*>(p.basis16 + (int64_t)w.cur.h * HEAD_DIM * RANK);
+    for (int o = tid; o < 128 * (RANK / 8); o += T5_THREADS) {
+      const int c = o / (RANK / 8), i8 = o % (RANK / 8);
+      reinterpret_cast<uint4*>(bbuf0)[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
+    }
+  }
 
   // ---- prologue: zeroed operand rows, barriers, tensor memory ----
   for (int i = tid; i < (T5_STAGES + 2) * T5_QB_BYTES / 16; i += T5_THREADS) {
@@ -157,9 +172,6 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   __syncthreads();
   tc5::fence_after();
   const uint32_t tmem = sh->tmem_base;
-
-  Walker w;
-  w.init(cum, npg_sm, f_begin, g.h_kv);
 
   // Registers move from the softmax, value and service warps to the key warps: each group of four warps
   // resizes itself first thing in its branch.
@@ -566,9 +578,11 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
             }
             uint4* bd = reinterpret_cast<uint4*>(bbuf0 + (size_t)(w.seg & 1) * COEF_BYTES);
             const uint4* bs = reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK);
-            for (int o = lane; o < 128 * (RANK / 8); o += 32) {
-              const int c = o / (RANK / 8), i8 = o % (RANK / 8);
-              bd[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
+            if (WALK == WALK_ALL || w.seg > 0) {
+              for (int o = lane; o < 128 * (RANK / 8); o += 32) {
+                const int c = o / (RANK / 8), i8 = o % (RANK / 8);
+                bd[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
+              }
             }
           }
           if (lane == 0) sh->bsel[s] = w.seg & 1, sh->first[s] = (w.it - first_cur < 2) ? 1 : 0;
@@ -654,6 +668,7 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
     tc5::fence_after();
     tc5::dealloc(tmem, TM_COLS);
   }
+  if constexpr (WALK == WALK_OWN) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 static size_t t5_smem_bytes(int rank, int group, int batch, int walk) {
@@ -673,7 +688,21 @@ static int launch_t5(const K2bDecodeParams& prm, int grid, size_t smem, cudaStre
       return BMXK_ERR_CUDA;
     }
   }
-  k2b_decode_t5_kernel<RANK, GQ, WALK><<<grid, T5_THREADS, smem, s>>>(prm);
+  if (WALK == WALK_OWN && prm.walk.after_prefix) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3(T5_THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k2b_decode_t5_kernel<RANK, GQ, WALK>, prm);
+    if (e != cudaSuccess) {
+      set_error("bmxk_k2b_decode(tcgen05): %s", cudaGetErrorString(e));
+      return BMXK_ERR_CUDA;
+    }
+  } else {
+    k2b_decode_t5_kernel<RANK, GQ, WALK><<<grid, T5_THREADS, smem, s>>>(prm);
+  }
   return check_launch("bmxk_k2b_decode(tcgen05)");
 }
 template <int WALK>

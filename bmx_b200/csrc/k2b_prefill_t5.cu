@@ -131,13 +131,14 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   const int b = blockIdx.z, h = blockIdx.y, i0 = (n_blocks - 1 - (int)blockIdx.x / n_split) * PP;
   const int H = g.h_kv * G;
   // MODE_PREFIX: row m is query head m % G of the group's member i0 + m / G (any G up to 8; 128 - PP * G rows idle)
-  const int m0 = MODE == MODE_PREFIX ? p.group_start[b] : 0, n_members = MODE == MODE_PREFIX ? p.group_start[b + 1] - m0 : 0;
+  const int4 group = MODE == MODE_PREFIX ? reinterpret_cast<const int4*>(p.groups)[b] : make_int4(0, 0, b, 0);
+  const int m0 = group.x, n_members = group.y - group.x, first_member = group.z;
+  if (MODE == MODE_PREFIX) asm volatile("griddepcontrol.launch_dependents;");  // the kernel that streams the pages behind the prefixes
   if (MODE == MODE_PREFIX && i0 >= n_members) return;
-  const int first_member = MODE == MODE_PREFIX ? p.members[m0] : b;
 
   const int64_t pq_min = p.q_pos0 + i0;                                // first query position of the CTA
   const int64_t pq_max = p.q_pos0 + min(i0 + PP, p.n_q) - 1;           // last one
-  const int n_pg = MODE == MODE_PREFIX ? min(max(p.skip[first_member], 0), p.n_pages[first_member]) : p.n_pages[b];
+  const int n_pg = MODE == MODE_PREFIX ? min(max(group.w, 0), p.n_pages[first_member]) : p.n_pages[b];
   const int64_t vis = MODE == MODE_PREFIX ? (int64_t)n_pg * 128 : pq_max - p.pos_offset;
   if (MODE != MODE_CAUSAL && FRAG && tid == 0 && min((int64_t)n_pg, vis / 128 + 1) > p.rope_pages && atomicCAS(p.status, 0, 3) == 0)
     p.status[1] = p.rope_pages, p.status[2] = n_pg;
@@ -157,6 +158,15 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   const int NT = NP + NW;
   const int64_t page_pos0 = p.pos_offset + (int64_t)T0 * 128;  // position of the first key of this share (MODE_SLIDING: see page_of)
 
+  const int32_t* table = p.page_table + (int64_t)first_member * p.table_stride;
+  auto copy_tile = [&](int stage, int slot) {  // one thread: a page's coefficients and its block of this head
+    uint8_t* st = stage0 + (size_t)stage * STAGE_BYTES;
+    mbar_arrive_expect_tx(&sh->full[stage], (uint32_t)STAGE_BYTES);
+    bulk_g2s(st, reinterpret_cast<const uint8_t*>(p.coefs) + ((int64_t)slot * g.n_coef_heads + (g.n_coef_heads == 1 ? 0 : h)) * COEF_BYTES, COEF_BYTES,
+             &sh->full[stage]);
+    bulk_g2s(st + COEF_BYTES, p.pages + ((int64_t)slot * g.h_kv + h) * PB, PB, &sh->full[stage]);
+  };
+
   // ---- prologue: barriers, tensor memory, the operands that do not change (Q, basis, constant rows of V') ----
   if (tid == 0) {
     for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1);
@@ -165,6 +175,14 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     for (int e = 0; e < 2; ++e) sh->kcnt[e] = sh->klcnt[e] = sh->vcnt[e] = sh->scnt[e] = sh->pcnt[e] = 0;
     for (int e = 0; e < 4; ++e) sh->turn[e] = 0;
     fence_barrier_init();
+    fence_proxy_async();
+    // the first tiles travel while the operands that do not change are laid out
+    int slot[P5_STAGES];
+#pragma unroll
+    for (int s = 0; s < P5_STAGES; ++s) slot[s] = (s < NP) ? table[page_of(s)] : 0;
+#pragma unroll
+    for (int s = 0; s < P5_STAGES; ++s)
+      if (s < NP) copy_tile(s, slot[s]);
   }
   if (warp == 16) {
     tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
@@ -376,21 +394,27 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         }
         if (++s == P5_STAGES) s = 0, fp ^= 1u;
       } else {
-        // window tile: values as stored, transposed; tokens past the window's length are zero
-        const int t0 = (n - NP) * 128;
+        // window tile: values as stored, transposed; tokens past the window's length are zero (MODE_SLIDING: and those that no row of
+        // the block sees, so that no infinity in them meets a weight of 0).  The four warps of a half take 16-byte pieces of its rows, four
+        // lanes to a row and four rows' loads in flight (the role has 40 registers), and scatter their channels.
+        const int t0 = (n - NP) * 128 + 64 * cc, c8 = 4 * wq + (lane & 3), tr = lane >> 2;
+        uint8_t* vcol = vop + c8 * V_SBO + 8 * cc * 128 + tr * 2;  // channels 8 c8 .. + 7, token 64 cc + 8 i + tr
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          uint32_t w4[4];
+        for (int i0_ = 0; i0_ < 8; i0_ += 4) {
+          uint4 rows[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int ta = t0 + 64 * cc + 8 * i + 2 * j;
-            // (MODE_SLIDING: what no row of the block sees stays out, so that no infinity in it meets a weight of 0)
-            auto in = [&](int t) { return t < tl && (MODE != MODE_SLIDING || tail_pos0 + t >= lo_min || tail_pos0 + t < p.sinks); };
-            const __half a = in(ta) ? vt[(int64_t)ta * HEAD_DIM + ch] : __float2half_rn(0.f);
-            const __half c = in(ta + 1) ? vt[(int64_t)(ta + 1) * HEAD_DIM + ch] : __float2half_rn(0.f);
-            w4[j] = h2_as_u32(__halves2half2(a, c));
+          for (int i = 0; i < 4; ++i) {
+            const int t = t0 + 8 * (i0_ + i) + tr;
+            const bool in = t < tl && (MODE != MODE_SLIDING || tail_pos0 + t >= lo_min || tail_pos0 + t < p.sinks);
+            rows[i] = in ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
           }
-          *reinterpret_cast<uint4*>(vrow + (8 * cc + i) * 128) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w4[4] = {rows[i].x, rows[i].y, rows[i].z, rows[i].w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<uint16_t*>(vcol + (i0_ + i) * 128 + k * 16) = (uint16_t)(k & 1 ? w4[k >> 1] >> 16 : w4[k >> 1] & 0xFFFFu);
+          }
         }
         if ((ch >> 6) == cc) vinv[0] = __float2half_rn(1.f), vinv[8] = __float2half_rn(0.f);
       }
@@ -720,11 +744,9 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     if (warp == 16) {
       constexpr uint32_t ID_U1 = tc5::idesc_f16_f16(128, 128);
       const uint64_t d_stage = tc5::smem_desc(smem_u32(stage0), 128, AB_SBO), d_b = tc5::smem_desc(smem_u32(bop), 128, AB_SBO);
-      const int chd = (g.n_coef_heads == 1) ? 0 : h;
-      const int32_t* table = p.page_table + (int64_t)first_member * p.table_stride;
-      int nP = 0, nA = 0, sP = 0, sA = 0;
+      int nP = min(NP, P5_STAGES), nA = 0, sP = nP % P5_STAGES, sA = 0;  // the prologue issued the first copies
       uint32_t phA = 0;
-      int slot = (NP > 0) ? table[page_of(0)] : 0;  // page slot of the next copy, fetched one copy ahead
+      int slot = (nP < NP) ? table[page_of(nP)] : 0;  // page slot of the next copy, fetched one copy ahead
       while (ok && nA < NP) {
         bool progressed = false;
         const int kc0 = smem_load_acquire(&sh->kcnt[0]), kc1 = smem_load_acquire(&sh->kcnt[1]);
@@ -748,13 +770,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         }
         // ---- copy ----
         if (nP < NP && (nP < P5_STAGES || (kdone(nP - P5_STAGES) && vc >= 4 * (nP - P5_STAGES + 1)))) {
-          uint8_t* st = stage0 + (size_t)sP * STAGE_BYTES;
-          if (el) {
-            mbar_arrive_expect_tx(&sh->full[sP], (uint32_t)STAGE_BYTES);
-            bulk_g2s(st, reinterpret_cast<const uint8_t*>(p.coefs) + ((int64_t)slot * g.n_coef_heads + chd) * COEF_BYTES, COEF_BYTES,
-                     &sh->full[sP]);
-            bulk_g2s(st + COEF_BYTES, p.pages + ((int64_t)slot * g.h_kv + h) * PB, PB, &sh->full[sP]);
-          }
+          if (el) copy_tile(sP, slot);
           __syncwarp();
           ++nP;
           if (++sP == P5_STAGES) sP = 0;

@@ -40,11 +40,10 @@ struct PrefillParams {
   // MODE_SLIDING: a row at position x sees the keys of (x - window, x] and those below `sinks`; pages that no row of a block sees are
   // not touched
   int64_t window, sinks;
-  // MODE_PREFIX: single-token queries q (batch, heads, 128) of the sequences members[group_start[z] .. group_start[z + 1] - 1] over
-  // the first skip[first member] pages of the first member's page-table row, which all of them share
-  const int32_t* skip;
+  // MODE_PREFIX: single-token queries q (batch, heads, 128) of the sequences members[begin .. end - 1] over the first `pages` pages of
+  // the page-table row of `first` (one of them), which all share; groups[z] = {begin, end, first, pages}, 16-byte aligned
   const int32_t* members;
-  const int32_t* group_start;
+  const int32_t* groups;
 };
 constexpr int MODE_CAUSAL = 0, MODE_PREFIX = 1, MODE_SLIDING = 2;
 constexpr int ROPE_FRAG_UINT4 = 2048;  // per page: [cos, sin][chunk of 16 pairs][32 tokens x 4][half of the chunk][lane]

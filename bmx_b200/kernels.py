@@ -6,6 +6,7 @@ libbmxk.so and raises `BmxkError` on a non-zero status.  Nothing in this module 
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 import functools
@@ -65,14 +66,27 @@ def _require_cuda(*ts: torch.Tensor) -> None:
             raise RuntimeError("bmxk kernels take CUDA tensors; there is no CPU path")
 
 
+_NO_CHANGE = contextlib.nullcontext()
+
+
 def _on_device_of(*ts: torch.Tensor | None):
     """The context in which a call on these tensors runs: their device, one for all of them, made current if it is not."""
-    _require_cuda(*ts)
-    devices = {t.device.index for t in ts if t is not None}
-    if len(devices) != 1:
-        raise RuntimeError(f"tensors of one call lie on different devices: {sorted(devices)}")
-    index = devices.pop()
-    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
+    index = None
+    for t in ts:
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if i < 0:
+                    raise RuntimeError("bmxk kernels take CUDA tensors; there is no CPU path")
+                if index is not None:
+                    raise RuntimeError(f"tensors of one call lie on different devices: {index} and {i}")
+                index = i
+    return _NO_CHANGE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _addr(t: torch.Tensor | None):
+    """Address of a tensor's first element as the plain integer ctypes converts fastest; None stays None."""
+    return None if t is None else t.data_ptr()
 
 
 def _require_device_visible(*ts: torch.Tensor) -> None:
@@ -359,24 +373,24 @@ def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_page
                 tail_len: torch.Tensor | None, signs: torch.Tensor) -> int:
     """What every step over a k2b pool asks of its tensors; returns the window's capacity."""
     g = pool.geom
-    batch = q.shape[0]
-    assert q.dtype == torch.float16 and q.is_contiguous() and q.shape[1] == g.h_kv * g.n_q_groups and q.shape[-1] == HEAD_DIM
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == batch and page_table.stride(1) == 1
-    assert n_pages.dtype == torch.int32 and n_pages.shape == (batch,) and n_pages.is_contiguous()
+    h_kv, batch, half, i32 = g.h_kv, q.shape[0], torch.float16, torch.int32
+    assert q.dtype is half and q.is_contiguous() and q.shape[1] == h_kv * g.n_q_groups and q.shape[-1] == HEAD_DIM
+    assert page_table.dtype is i32 and page_table.dim() == 2 and page_table.shape[0] == batch and page_table.stride(1) == 1
+    assert n_pages.dtype is i32 and n_pages.dim() == 1 and n_pages.numel() == batch and n_pages.is_contiguous()
     assert 0 <= max_pages <= page_table.shape[1], f"max_pages={max_pages}: the page table has {page_table.shape[1]} columns"
-    assert signs.dtype == torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
+    assert signs.dtype is torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
     if max_pages > 0:
-        assert basis_f16.dtype == torch.float16 and basis_f16.shape == (g.h_kv * HEAD_DIM, g.rank) and basis_f16.is_contiguous()
+        assert basis_f16.dtype is half and basis_f16.is_contiguous() and basis_f16.numel() == h_kv * HEAD_DIM * g.rank
         for t in (rope_cos, rope_sin):
-            assert t.dtype == torch.float16 and t.is_contiguous() and t.shape[1] == HEAD_DIM and t.shape[0] >= 128
+            assert t.dtype is half and t.is_contiguous() and t.shape[1] == HEAD_DIM and t.shape[0] >= 128
     if k_tail is None:
         assert v_tail is None and tail_len is None
         return 0
-    tail_cap = k_tail.shape[2]
-    assert k_tail.dtype == v_tail.dtype == torch.float16 and k_tail.is_contiguous() and v_tail.is_contiguous()
-    assert k_tail.shape == (batch, g.h_kv, tail_cap, HEAD_DIM) == v_tail.shape
-    assert tail_len.dtype == torch.int32 and tail_len.shape == (batch,) and tail_len.is_contiguous()
-    return tail_cap
+    shape = k_tail.shape
+    assert k_tail.dtype is half and v_tail.dtype is half and k_tail.is_contiguous() and v_tail.is_contiguous()
+    assert len(shape) == 4 and shape[0] == batch and shape[1] == h_kv and shape[3] == HEAD_DIM and v_tail.shape == shape
+    assert tail_len.dtype is i32 and tail_len.dim() == 1 and tail_len.numel() == batch and tail_len.is_contiguous()
+    return shape[2]
 
 
 def _check_out(out: torch.Tensor | None, q: torch.Tensor, dtypes: tuple) -> torch.Tensor:
@@ -399,9 +413,9 @@ def k2b_decode_sliding(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, 
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs, workspace):
         tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
         out = _check_out(out, q, (torch.float16, torch.float32))
-        call("bmxk_k2b_decode_sliding", ctypes.byref(g), _ptr(q), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16), _ptr(page_table),
-             page_table.stride(0), _ptr(n_pages), q.shape[0], max_pages, _ptr(rope_cos), _ptr(rope_sin), _ptr(k_tail), _ptr(v_tail), _ptr(tail_len),
-             tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), int(window), int(sinks), _ptr(workspace), workspace.numel(), _ptr(out),
+        call("bmxk_k2b_decode_sliding", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
+             page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(rope_cos), _addr(rope_sin), _addr(k_tail), _addr(v_tail), _addr(tail_len),
+             tail_cap, _addr(v_lut), _addr(signs), sm_scale, int(window), int(sinks), _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
     return out
 
@@ -429,10 +443,10 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
             n_split = split_walk(ctas, seen, q.device, 16)
         nbytes = int(_lib.lib().bmxk_k2b_prefill_workspace_bytes(ctypes.byref(g), n_q, batch, int(n_split)))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        call("bmxk_k2b_prefill_sliding", ctypes.byref(g), _ptr(q), n_q, int(q_pos0), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16),
-             _ptr(page_table), page_table.stride(0), _ptr(n_pages), batch, _ptr(rope_cos), _ptr(rope_sin), _ptr(rope), rope_pages, _ptr(k_tail),
-             _ptr(v_tail), _ptr(tail_len), tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), int(window), int(sinks), _ptr(status),
-             _ptr(out), int(n_split), _ptr(ws), nbytes, _stream())
+        call("bmxk_k2b_prefill_sliding", ctypes.byref(g), _addr(q), n_q, int(q_pos0), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16),
+             _addr(page_table), page_table.stride(0), _addr(n_pages), batch, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail),
+             _addr(v_tail), _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, int(window), int(sinks), _addr(status),
+             _addr(out), int(n_split), _addr(ws), nbytes, _stream())
     return out
 
 
@@ -456,15 +470,16 @@ class PrefixGroups:
             raise ValueError(f"a batch row is in one group at most and below {batch}: {members}")
         if any(p < 0 for p in prefix_pages):
             raise ValueError(f"prefix_pages {prefix_pages}")
-        skip, start = [0] * batch, [0]
+        skip, info, begin = [0] * batch, [], 0
         for m, p in zip(members, prefix_pages):
-            start.append(start[-1] + len(m))
+            info += [begin, begin + len(m), int(m[0]) if len(m) else 0, int(p)]
+            begin += len(m)
             for r in m:
                 skip[int(r)] = int(p)
         self.batch, self.n_groups, self.max_members = batch, len(members), max((len(m) for m in members), default=0)
         self.max_prefix = max(prefix_pages, default=0)
-        packed = torch.tensor(skip + start + rows, dtype=torch.int32).to(device)
-        self.skip, self.group_start, self.members = packed[:batch], packed[batch:batch + len(start)], packed[batch + len(start):]
+        packed = torch.tensor(info + skip + rows, dtype=torch.int32).to(device)
+        self.info, self.skip, self.members = packed[:len(info)], packed[len(info):len(info) + batch], packed[len(info) + batch:]
         pp = 128 // g.n_q_groups
         ctas = g.h_kv * sum(-(-len(m) // pp) for m, p in zip(members, prefix_pages) if p)
         self.n_split = n_split if n_split is not None else split_walk(max(1, ctas), max(1, self.max_prefix), device)
@@ -491,10 +506,10 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
         assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
         rope_pages = _check_fragments(rope, groups.max_prefix)
         out = _check_out(out, q, (torch.float16, torch.float32))
-        call("bmxk_k2b_decode_shared", ctypes.byref(g), _ptr(q), _ptr(pool.pages), _ptr(pool.coefs), _ptr(basis_f16), _ptr(page_table),
-             page_table.stride(0), _ptr(n_pages), q.shape[0], max_pages, _ptr(groups.skip), _ptr(groups.members), _ptr(groups.group_start),
-             groups.n_groups, groups.max_members, groups.n_split, _ptr(rope_cos), _ptr(rope_sin), _ptr(rope), rope_pages, _ptr(k_tail), _ptr(v_tail),
-             _ptr(tail_len), tail_cap, _ptr(v_lut), _ptr(signs), ctypes.c_float(sm_scale), _ptr(workspace), workspace.numel(), _ptr(out),
+        call("bmxk_k2b_decode_shared", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
+             page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
+             groups.n_groups, groups.max_members, groups.n_split, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail), _addr(v_tail),
+             _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
     return out
 
@@ -610,26 +625,33 @@ def window_shift(k_win: torch.Tensor, v_win: torch.Tensor, k_src_win: torch.Tens
          _ptr(n_pages), int(pages_added), _stream())
 
 
-def _slot_list(slots) -> torch.Tensor:
-    t = slots if isinstance(slots, torch.Tensor) else torch.tensor(slots, dtype=None if len(slots) else torch.int64)
-    if t.is_cuda or t.dim() != 1 or t.is_floating_point() or t.dtype == torch.bool:
-        raise TypeError("copy_slots: slots are a list of integers or a 1-D integer tensor on the host")
-    if t.dtype != torch.int32:
-        if t.numel() and (int(t.min()) < -(1 << 31) or int(t.max()) >= 1 << 31):
-            raise ValueError("copy_slots: a slot does not fit 32 bits")
-        t = t.to(torch.int32)
-    return t.contiguous()
+def _slot_list(slots):
+    """(object that keeps the memory, address, length) of a list of slots as int32 on the host."""
+    if isinstance(slots, torch.Tensor):
+        if slots.is_cuda or slots.dim() != 1 or slots.is_floating_point() or slots.is_complex() or slots.dtype == torch.bool:
+            raise TypeError("copy_slots: slots are a list of integers or a 1-D integer tensor on the host")
+        if slots.dtype != torch.int32:
+            if slots.numel() and (int(slots.min()) < -(1 << 31) or int(slots.max()) >= 1 << 31):
+                raise ValueError("copy_slots: a slot does not fit 32 bits")
+            slots = slots.to(torch.int32)
+        slots = slots.contiguous()
+        return slots, slots.data_ptr(), slots.numel()
+    try:
+        held = array.array("i", slots)
+    except OverflowError:
+        raise ValueError("copy_slots: a slot does not fit 32 bits") from None
+    return (held, *held.buffer_info())
 
 
 def _slot_bytes(t: torch.Tensor) -> tuple[int, int]:
     """(bytes of one slot, bytes from slot to slot) of an array whose first dimension counts slots."""
-    n = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size != 1 and stride != n:
-            raise ValueError(f"copy_slots: the values of a slot must lie in one piece, strides {t.stride()} for shape {tuple(t.shape)}")
-        n *= size
+    shape, strides, n = t.shape, t.stride(), 1
+    for d in range(len(shape) - 1, 0, -1):
+        if strides[d] != n and shape[d] != 1:
+            raise ValueError(f"copy_slots: the values of a slot must lie in one piece, strides {strides} for shape {tuple(shape)}")
+        n *= shape[d]
     item = t.element_size()
-    return n * item, (t.stride(0) if t.shape[0] > 1 else n) * item
+    return n * item, (strides[0] if shape[0] > 1 else n) * item
 
 
 def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
@@ -641,22 +663,26 @@ def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
     must not write a slot that it reads, and no slot may be written twice: both are refused, like indices out of range."""
     if len(srcs) != len(dsts) or not 1 <= len(srcs) <= 8:
         raise ValueError(f"copy_slots: {len(srcs)} sources and {len(dsts)} destinations (1 to 8 of each)")
+    n, n_src, n_dst = len(srcs), srcs[0].shape[0], dsts[0].shape[0]
+    sizes = []
     for s, d in zip(srcs, dsts):
         if s.dtype != d.dtype or s.dim() < 2 or s.shape[1:] != d.shape[1:]:
             raise ValueError(f"copy_slots: {tuple(s.shape)} {s.dtype} cannot be copied to {tuple(d.shape)} {d.dtype}")
-        if s.shape[0] != srcs[0].shape[0] or d.shape[0] != dsts[0].shape[0]:
+        if s.shape[0] != n_src or d.shape[0] != n_dst:
             raise ValueError("copy_slots: arrays of one call have the same number of slots")
-    a, b = _slot_list(src_slots), _slot_list(dst_slots)
-    if a.numel() != b.numel():
-        raise ValueError(f"copy_slots: {a.numel()} slots to read and {b.numel()} to write")
-    if a.numel() == 0:
+        size, src_stride = _slot_bytes(s)
+        sizes.append((s.data_ptr(), d.data_ptr(), src_stride, src_stride if d is s else _slot_bytes(d)[1], size))
+    a, a_at, a_n = _slot_list(src_slots)
+    b, b_at, b_n = _slot_list(dst_slots)
+    if a_n != b_n:
+        raise ValueError(f"copy_slots: {a_n} slots to read and {b_n} to write")
+    if a_n == 0:
         return
-    n = len(srcs)
-    src_bytes, dst_bytes = [_slot_bytes(t) for t in srcs], [_slot_bytes(t) for t in dsts]
+    # the five host arrays of the call in one block of 64-bit words: sources, destinations, their strides, sizes
+    words = array.array("q", [x[k] for k in range(5) for x in sizes])
+    at = words.buffer_info()[0]
     with _on_device_of(*srcs, *dsts):
-        call("bmxk_copy_slots", n, (ctypes.c_void_p * n)(*(t.data_ptr() for t in srcs)), (ctypes.c_void_p * n)(*(t.data_ptr() for t in dsts)),
-             (ctypes.c_int64 * n)(*(x[1] for x in src_bytes)), (ctypes.c_int64 * n)(*(x[1] for x in dst_bytes)),
-             (ctypes.c_int64 * n)(*(x[0] for x in src_bytes)), _ptr(a), _ptr(b), a.numel(), srcs[0].shape[0], dsts[0].shape[0], _stream())
+        call("bmxk_copy_slots", n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, a_at, b_at, a_n, n_src, n_dst, _stream())
 
 
 def step_ingest(q_src: torch.Tensor, q_dst: torch.Tensor, k_post: torch.Tensor, v: torch.Tensor, k_src: torch.Tensor,

@@ -157,11 +157,11 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
                             const uint32_t* v_lut, const float* signs, float sm_scale, int64_t window, int64_t sinks, void* workspace,
                             size_t workspace_bytes, void* out, int out_dtype, void* stream);
 
-/* One decode step for sequences that share prefixes of whole pages: group z is the sequences members[group_start[z]] ..
- * members[group_start[z + 1] - 1] (each sequence in one group at most), whose page-table rows begin with the same skip[s] entries
- * (skip[s] = 0 for a sequence in no group).  A group's prefix is dequantized once for 128 / n_q_groups sequences at a time and its
+/* One decode step for sequences that share prefixes of whole pages.  groups[z] = {begin, end, first, pages} (int32 x 4, 16-byte aligned):
+ * the sequences members[begin] .. members[end - 1] (each in one group at most) have page-table rows that begin with the same `pages`
+ * entries, read from the row of `first`, one of them; skip[s] = pages for them and 0 for a sequence in no group.  A group's prefix is dequantized once for 128 / n_q_groups sequences at a time and its
  * pages are shared out over n_split CTAs; the pages behind it, the fp16 window and the merge are those of bmxk_k2b_decode, whose
- * arguments and result these are (no pos_offset, no partial states).  skip, members, group_start: int32 device arrays; max_members: the
+ * arguments and result these are (no pos_offset, no partial states).  skip, members, groups: int32 device arrays; max_members: the
  * largest group.  rope_frag: bmxk_k2b_rope_fragments of rope_pages pages (every prefix has to lie within, see the status word (3,
  * rope_pages, pages)), or null: the tables are read as they are, about a quarter slower.  Layout 1, sm_scale > 0.  workspace:
  * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once.  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every
@@ -169,7 +169,7 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
 size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split);
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
                            const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
-                           const int32_t* members, const int32_t* group_start, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
                            const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
                            const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
                            size_t workspace_bytes, void* out, int out_dtype, void* stream);

@@ -94,3 +94,10 @@ def coefs(pool):
     """Coefficients (slots, coef heads, token / 8, rank / 8, token % 8, 8) as they lie in the coefficient blocks of layout 1."""
     g = pool.geom
     return pool.coefs.view(torch.float16).view(pool.n_slots, g.n_coef_heads, 16, g.rank // 8, 8, 8)
+
+
+def assert_one_step(a, b):
+    """Two fp16 outputs of the same float32 values summed in another order: the sums differ by a few float32 roundings (1e-5 of the row's
+    largest entry covers 2^7 of them), the rounded values by one fp16 step at most (2^-10 relative) where that crosses a border."""
+    a, b = a.detach().cpu().double(), b.detach().cpu().double()
+    assert ((a - b).abs() <= 2.0 ** -10 * a.abs().maximum(b.abs()) + 1e-5 * a.abs().amax(-1, keepdim=True) + 2.0 ** -24).all()

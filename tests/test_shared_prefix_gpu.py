@@ -100,7 +100,7 @@ def test_no_groups_equals_the_plain_step_and_empty_sequences_give_zero():
     w = World(K, _dev(), [], [(5, 60), (1, 1), (9, 150)])
     plain = K.k2b_decode(w.pool, w.q, w.basis, w.table, w.n_pages, w.max_pages, w.cos, w.sin, w.k_win, w.v_win, w.tail_len, w.v_lut, w.signs, 1 / math.sqrt(D),
                          K.decode_workspace(w.geom, 3, w.max_pages, w.q.device))
-    assert torch.equal(w.decode(K), plain)
+    P.assert_one_step(w.decode(K), plain)
     w = World(K, _dev(), [(3, [(0, 9)] * 3)], [(0, 0)])
     out = w.decode(K)
     P.assert_attention(out, w.ref)

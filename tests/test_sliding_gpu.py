@@ -148,7 +148,7 @@ def test_decode_equals_the_plain_step_when_everything_is_visible():
     w = World(K, _dev(), [1500, 700, 64, 193], 10 ** 9, 0)
     plain = K.k2b_decode(w.pool, w.q[:, :, 0].contiguous(), w.basis, w.table, w.n_pages, w.max_pages, w.cos, w.sin, w.k_win, w.v_win, w.tail_len, w.v_lut,
                          w.signs, 1 / math.sqrt(D), K.decode_workspace(w.geom, 4, w.max_pages, w.q.device))
-    assert torch.equal(w.decode(K), plain)
+    P.assert_one_step(w.decode(K), plain)
 
 
 @pytest.mark.gpu
