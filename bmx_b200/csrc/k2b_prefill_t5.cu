@@ -168,54 +168,59 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   };
 
   // ---- prologue: barriers, tensor memory, the operands that do not change (Q, basis, constant rows of V') ----
-  if (tid == 0) {
-    for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1);
-    mbar_init(&sh->low, 1);
-    for (int e = 0; e < 2; ++e) mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1);
-    for (int e = 0; e < 2; ++e) sh->kcnt[e] = sh->klcnt[e] = sh->vcnt[e] = sh->scnt[e] = sh->pcnt[e] = 0;
-    for (int e = 0; e < 4; ++e) sh->turn[e] = 0;
-    fence_barrier_init();
-    fence_proxy_async();
-    // the first tiles travel while the operands that do not change are laid out
-    int slot[P5_STAGES];
-#pragma unroll
-    for (int s = 0; s < P5_STAGES; ++s) slot[s] = (s < NP) ? table[page_of(s)] : 0;
-#pragma unroll
-    for (int s = 0; s < P5_STAGES; ++s)
-      if (s < NP) copy_tile(s, slot[s]);
-  }
+  // (warp 16: barriers, the first copies and tensor memory; the others: the operands)
   if (warp == 16) {
+    if (lane == 0) {
+      for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->low, 1);
+      for (int e = 0; e < 2; ++e) mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1);
+      for (int e = 0; e < 2; ++e) sh->kcnt[e] = sh->klcnt[e] = sh->vcnt[e] = sh->scnt[e] = sh->pcnt[e] = 0;
+      for (int e = 0; e < 4; ++e) sh->turn[e] = 0;
+      fence_barrier_init();
+      fence_proxy_async();
+      // the first tiles travel while the operands that do not change are laid out
+      int slot[P5_STAGES];
+#pragma unroll
+      for (int s = 0; s < P5_STAGES; ++s) slot[s] = (s < NP) ? table[page_of(s)] : 0;
+#pragma unroll
+      for (int s = 0; s < P5_STAGES; ++s)
+        if (s < NP) copy_tile(s, slot[s]);
+    }
+    __syncwarp();
     tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
     tc5::relinquish();
-  }
-  for (int o = tid; o < 128 * 18; o += P5_THREADS) {  // row m = (query head m / PP, position i0 + m % PP)
-    const int m = o / 18, c8 = o % 18;
-    const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
-    uint4 v = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
-    if (c8 < 16) {
-      const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
-      v = reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM)[c8];
+  } else {
+    constexpr int ST = P5_THREADS - 32;
+    const int st = tid - (warp > 16 ? 32 : 0);
+    for (int o = st; o < 128 * 18; o += ST) {  // row m = (query head m / PP, position i0 + m % PP)
+      const int m = o / 18, c8 = o % 18;
+      const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
+      uint4 v = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
+      if (c8 < 16) {
+        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+        v = reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM)[c8];
+      }
+      *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = v;
+      if (c8 == 17) {  // K index 136 .. 143 of both key buffers: zero for good
+        *reinterpret_cast<uint4*>(kop0 + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(kop0 + OP_BYTES + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
     }
-    *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = v;
-    if (c8 == 17) {  // K index 136 .. 143 of both key buffers: zero for good
-      *reinterpret_cast<uint4*>(kop0 + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-      *reinterpret_cast<uint4*>(kop0 + OP_BYTES + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    {
+      uint4* bd = reinterpret_cast<uint4*>(bop);
+      const uint4* bs = reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK);
+      for (int o = st; o < 128 * (RANK / 8); o += ST) {
+        const int c = o / (RANK / 8), i8 = o % (RANK / 8);
+        bd[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
+      }
     }
-  }
-  {
-    uint4* bd = reinterpret_cast<uint4*>(bop);
-    const uint4* bs = reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK);
-    for (int o = tid; o < 128 * (RANK / 8); o += P5_THREADS) {
-      const int c = o / (RANK / 8), i8 = o % (RANK / 8);
-      bd[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
+    for (int o = st; o < 16 * 16; o += ST) {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
+      const int r = 128 + (o >> 4), i = o & 15;
+      const uint32_t w = (r == 130) ? 0x3C003C00u : 0u;
+      *reinterpret_cast<uint4*>(vop + (r >> 3) * V_SBO + i * 128 + (r & 7) * 16) = make_uint4(w, w, w, w);
     }
+    if (st < 128) sg[st] = p.signs[st] * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
   }
-  for (int o = tid; o < 16 * 16; o += P5_THREADS) {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
-    const int r = 128 + (o >> 4), i = o & 15;
-    const uint32_t w = (r == 130) ? 0x3C003C00u : 0u;
-    *reinterpret_cast<uint4*>(vop + (r >> 3) * V_SBO + i * 128 + (r & 7) * 16) = make_uint4(w, w, w, w);
-  }
-  if (tid < 128) sg[tid] = p.signs[tid] * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
   fence_proxy_async();
   tc5::fence_before();
   __syncthreads();
@@ -635,6 +640,9 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         tc5::wait_ld();
         lsum = __uint_as_float(r4[0]) + __uint_as_float(r4[1]), add = p.lut_alpha * __uint_as_float(r4[2]);
       }
+      // a row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used) and
+      // leave 512 bytes at a time (16 bytes of 32 rows per store kept the store unit busy for 2 us)
+      float* stage = reinterpret_cast<float*>(kop0) + (size_t)wq * 32 * PREFIX_PART_STRIDE;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t r[32];
@@ -647,10 +655,16 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
 #pragma unroll
           for (int i = 0; i < 32; ++i) r[i] = 0u;
         }
-        if (live) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(rec + 32 * c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-        }
+        for (int j = 0; j < 8; ++j)
+          reinterpret_cast<uint4*>(stage + lane * PREFIX_PART_STRIDE + 32 * c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+      }
+      __syncwarp();
+      const uint64_t rec_u = live ? reinterpret_cast<uint64_t>(rec) : 0;
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) {
+        float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, rec_u, i));
+        if (dst) reinterpret_cast<float4*>(dst)[lane] = reinterpret_cast<const float4*>(stage + i * PREFIX_PART_STRIDE)[lane];
       }
       if (live) *reinterpret_cast<float4*>(rec + 128) = make_float4(NT > 0 ? m : -INFINITY, lsum, 0.f, 0.f);
     } else if (alive) {
@@ -691,28 +705,34 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         }
         if (ip < p.n_q) *reinterpret_cast<float4*>(rec + 128) = make_float4(m, lsum, 0.f, 0.f);
       } else {
-      uint4* dst = reinterpret_cast<uint4*>(p.out + grow * HEAD_DIM);
+        // through shared memory, as above: two rows of 256 bytes per store
+        uint4* stage = reinterpret_cast<uint4*>(kop0) + (size_t)wq * 32 * 17;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        if (NT > 0) {
-          tc5::ld32(tl_ + TM_O + 32 * c, r);
-          tc5::wait_ld();
-        } else {
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          if (NT > 0) {
+            tc5::ld32(tl_ + TM_O + 32 * c, r);
+            tc5::wait_ld();
+          } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
-        }
-        if (ip < p.n_q) {
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t w4[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w4[i] = pack_h2(__uint_as_float(r[8 * j + 2 * i]) * inv, __uint_as_float(r[8 * j + 2 * i + 1]) * inv);
-            dst[4 * c + j] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            stage[lane * 17 + 4 * c + j] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
         }
-      }
+        __syncwarp();
+        const int64_t mine = ip < p.n_q ? grow : -1;
+#pragma unroll 4
+        for (int i = 0; i < 32; i += 2) {
+          const int64_t to = __shfl_sync(0xffffffffu, mine, i + (lane >> 4));
+          if (to >= 0) reinterpret_cast<uint4*>(p.out + to * HEAD_DIM)[lane & 15] = stage[(i + (lane >> 4)) * 17 + (lane & 15)];
+        }
       }
     }
   } else {
@@ -780,23 +800,25 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         if (stalled(progressed, 40)) ok = false;
       }
     } else if (warp == 17) {
-      constexpr uint32_t ID_U2 = tc5::idesc_f16_f32(128, 64);
+      // one contraction per tile: the rows of Q are read from shared memory once for its 128 keys (twice per tile in halves of 64, which
+      // made U2 wait for shared memory); each half's softmax warps have a barrier of their own
+      constexpr uint32_t ID_U2 = tc5::idesc_f16_f32(128, 128);
       const uint64_t d_q = tc5::smem_desc(smem_u32(qop), 128, OP_SBO), d_k = tc5::smem_desc(smem_u32(kop0), 128, OP_SBO);
-      int uB = 0;  // half tiles issued
-      while (ok && uB < 2 * NT) {
-        const int n = uB >> 1, hf = uB & 1;
-        const int kc = smem_load_acquire(&sh->kcnt[n & 1]), sc = smem_load_acquire(&sh->scnt[hf]);
+      int n = 0;  // tiles issued
+      while (ok && n < NT) {
+        const int kc = smem_load_acquire(&sh->kcnt[n & 1]), sc = min(smem_load_acquire(&sh->scnt[0]), smem_load_acquire(&sh->scnt[1]));
         bool progressed = false;
         if (kc >= 8 * ((n >> 1) + 1) && sc >= 4 * n) {
           tc5::fence_after();
-          const uint64_t db = d_k + (uint64_t)((n & 1) * (OP_BYTES >> 4) + hf * (8 * OP_SBO >> 4));  // token rows 64 hf ..
+          const uint64_t db = d_k + (uint64_t)((n & 1) * (OP_BYTES >> 4));
           if (el) {
 #pragma unroll
-            for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S + 64 * hf, d_q + 16 * ks, db + 16 * ks, ID_U2, ks > 0);  // 144 channels
-            tc5::commit(smem_u32(&sh->sdone[hf][n & 1]));
+            for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S, d_q + 16 * ks, db + 16 * ks, ID_U2, ks > 0);  // 144 channels
+            tc5::commit(smem_u32(&sh->sdone[0][n & 1]));
+            tc5::commit(smem_u32(&sh->sdone[1][n & 1]));
           }
           __syncwarp();
-          ++uB;
+          ++n;
           progressed = true;
         }
         if (stalled(progressed, 51)) ok = false;
