@@ -35,6 +35,8 @@
 // the rotation is undone, running maximum, sum of weights) and a small kernel merges them.
 //
 // Every wait is bounded and reports through the status words; nothing here waits on another CTA.
+#include <type_traits>
+
 #include "prefill_common.cuh"
 #include "tc5.cuh"
 
@@ -42,7 +44,7 @@ namespace bmxk {
 
 namespace {
 
-constexpr int P5_THREADS = 896;  // warps 0-7 key, 8-15 softmax (8-11 first halves, 12-15 second halves), 16 copies + U1, 17 U2, 18 U3 (19 idle), 20-27 value
+constexpr int P5_THREADS = 896;  // warps 0-7 key, 8-15 softmax (8-11 first halves, 12-15 second halves), 16 U1, 17 U2, 18 U3, 19 copies, 20-27 value
 constexpr int P5_STAGES = 3;
 // Registers per thread after each group of four warps resizes itself; the pool is what the launch handed out.
 constexpr int P5_REG_LAUNCH = 72, P5_REG_KEY = 96, P5_REG_SOFTMAX = 96, P5_REG_SERVICE = 40, P5_REG_VALUE = 40;
@@ -59,15 +61,16 @@ constexpr float MIN_NORM = 9.765625e-4f;  // 2^-10: a zero value vector keeps a 
 // TMEM columns: scores (64 per half of a tile), weights (fp16 pairs, 32 per half), output accumulator (128 channels, sum of p in two parts, sum of p x norm, 13 unused), K_low
 constexpr uint32_t TM_S = 0, TM_P = 128, TM_O = 192, TM_KL = 336, TM_COLS = 512;
 
+// Every hand-over is an mbarrier: a warp that waits on one is parked by the hardware and takes no issue slots.  (Counters in shared memory
+// polled with acquiring loads cost the issuing warps 400 - 1300 cycles per look, a good part of a tile's 3200.)
 struct P5Smem {
-  uint64_t full[P5_STAGES];          // raw tile landed (bulk copies)
-  uint64_t low, sdone[2][2], odone[2];  // completion of U1, of U2 [half][tile parity] and of U3 [half] (tcgen05.commit)
+  uint64_t full[P5_STAGES], empty[P5_STAGES];  // raw tile landed (bulk copies); read by the key and value warps (16 arrivals)
+  uint64_t low, sdone[2][2], odone[2];         // completion of U1, of U2 [half][tile parity] and of U3 [half] (tcgen05.commit)
+  uint64_t keys[2], klow;                      // key warps (8): keys of the tile written [tile parity]; K_low in registers (U1 of the next may start)
+  uint64_t values[2], scores[2], weights[2];   // per half (4 warps): value operand written, scores read, weights written
+  uint64_t turn[2][4];                         // [half][group of 32 rows]: the half's running maximum is settled (the two warps of a group alternate)
+  uint64_t rot[4];                             // steps of the inverse value rotation that both warps of a group are through
   uint32_t tmem_base;
-  // Arrivals, never reset: key warps (8 per tile, counted per tile parity: a key warp may be two tiles ahead of another
-  // one, never two tiles of the same parity); per half: value warps, scores read, weights written (4 each per tile)
-  // klcnt: key warps that hold K_low of the tile in registers (U1 of the next tile may start)
-  // turn: half tiles whose running maximum is settled, per group of 32 rows (the two softmax warps of a group alternate)
-  int kcnt[2], klcnt[2], vcnt[2], scnt[2], pcnt[2], turn[4];
   float m[128];  // the running maximum of each row, valid for the halves settled so far
 };
 
@@ -168,14 +171,17 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   };
 
   // ---- prologue: barriers, tensor memory, the operands that do not change (Q, basis, constant rows of V') ----
-  // (warp 16: barriers, the first copies and tensor memory; the others: the operands)
+  // (warp 16: barriers and the first copies; the others: the operands; warp 17 also tensor memory)
   if (warp == 16) {
     if (lane == 0) {
-      for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->low, 1);
-      for (int e = 0; e < 2; ++e) mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1);
-      for (int e = 0; e < 2; ++e) sh->kcnt[e] = sh->klcnt[e] = sh->vcnt[e] = sh->scnt[e] = sh->pcnt[e] = 0;
-      for (int e = 0; e < 4; ++e) sh->turn[e] = 0;
+      for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 16);
+      mbar_init(&sh->low, 1), mbar_init(&sh->klow, 8);
+      for (int e = 0; e < 2; ++e) {
+        mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1), mbar_init(&sh->keys[e], 8);
+        mbar_init(&sh->values[e], 4), mbar_init(&sh->scores[e], 4), mbar_init(&sh->weights[e], 4);
+        for (int w = 0; w < 4; ++w) mbar_init(&sh->turn[e][w], 1);
+      }
+      for (int w = 0; w < 4; ++w) mbar_init(&sh->rot[w], 2);
       fence_barrier_init();
       fence_proxy_async();
       // the first tiles travel while the operands that do not change are laid out
@@ -187,39 +193,48 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         if (s < NP) copy_tile(s, slot[s]);
     }
     __syncwarp();
-    tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
-    tc5::relinquish();
   } else {
-    constexpr int ST = P5_THREADS - 32;
+    // every load of a thread is in flight before its first store
+    constexpr int ST = P5_THREADS - 32, NQ = (128 * 18 + ST - 1) / ST;
     const int st = tid - (warp > 16 ? 32 : 0);
-    for (int o = st; o < 128 * 18; o += ST) {  // row m = (query head m / PP, position i0 + m % PP)
-      const int m = o / 18, c8 = o % 18;
-      const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
-      uint4 v = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
-      if (c8 < 16) {
-        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
-        v = reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM)[c8];
+    if (warp == 17) {
+      tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
+      tc5::relinquish();
+    }
+    uint4 qv[NQ];
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {  // row m = (query head m / PP, position i0 + m % PP)
+      const int o = st + i * ST, m = o / 18, c8 = o % 18;
+      qv[i] = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
+      if (c8 < 16 && m < 128) {
+        const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
+        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)__ldg(p.members + m0 + ip) * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+        qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM) + c8);
       }
-      *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = v;
+    }
+    const uint4 bv = st < 128 * (RANK / 8) ? __ldg(reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK) + st) : make_uint4(0u, 0u, 0u, 0u);
+    static_assert(128 * (32 / 8) <= ST, "one piece of the basis per thread");
+    const float sv = st < 128 ? __ldg(p.signs + st) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int o = st + i * ST, m = o / 18, c8 = o % 18;
+      if (m >= 128) break;
+      *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = qv[i];
       if (c8 == 17) {  // K index 136 .. 143 of both key buffers: zero for good
         *reinterpret_cast<uint4*>(kop0 + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(kop0 + OP_BYTES + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
       }
     }
-    {
-      uint4* bd = reinterpret_cast<uint4*>(bop);
-      const uint4* bs = reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK);
-      for (int o = st; o < 128 * (RANK / 8); o += ST) {
-        const int c = o / (RANK / 8), i8 = o % (RANK / 8);
-        bd[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bs[o];
-      }
+    if (st < 128 * (RANK / 8)) {
+      const int c = st / (RANK / 8), i8 = st % (RANK / 8);
+      reinterpret_cast<uint4*>(bop)[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bv;
     }
-    for (int o = st; o < 16 * 16; o += ST) {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
-      const int r = 128 + (o >> 4), i = o & 15;
+    if (st < 16 * 16) {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
+      const int r = 128 + (st >> 4), i = st & 15;
       const uint32_t w = (r == 130) ? 0x3C003C00u : 0u;
       *reinterpret_cast<uint4*>(vop + (r >> 3) * V_SBO + i * 128 + (r & 7) * 16) = make_uint4(w, w, w, w);
     }
-    if (st < 128) sg[st] = p.signs[st] * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
+    if (st < 128) sg[st] = sv * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
   }
   fence_proxy_async();
   tc5::fence_before();
@@ -297,7 +312,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
             PROF_ADD(3)
             tc5::fence_before();
             __syncwarp();
-            if (lane == 0) smem_add_release(&sh->klcnt[e], 1);
+            if (lane == 0) mbar_arrive(&sh->klow);
           }
 #pragma unroll
           for (int wd = 0; wd < 2; ++wd) {
@@ -333,6 +348,10 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
           *reinterpret_cast<uint4*>(krow + (8 + 2 * k) * 128) = make_uint4(out[8], out[9], out[10], out[11]);
           *reinterpret_cast<uint4*>(krow + (9 + 2 * k) * 128) = make_uint4(out[12], out[13], out[14], out[15]);
         }
+        if (n + P5_STAGES < NP) {  // its stage takes another tile
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->empty[s]);
+        }
         if (++s == P5_STAGES) s = 0, fp ^= 1u;
       } else {
         // window tile: the keys are stored rotated; rows past the window's length are zero; norm 1
@@ -350,7 +369,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) smem_add_release(&sh->kcnt[e], 1);
+      if (lane == 0) mbar_arrive(&sh->keys[e]);
       PROF_ADD(4)
     }
     PROF_OUT(16, 6)
@@ -397,6 +416,10 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
           const __half rh = __float2half_rn(r);
           vinv[0] = rh, vinv[8] = __float2half_rn(r - __half2float(rh));
         }
+        if (n + P5_STAGES < NP) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->empty[s]);
+        }
         if (++s == P5_STAGES) s = 0, fp ^= 1u;
       } else {
         // window tile: values as stored, transposed; tokens past the window's length are zero (MODE_SLIDING: and those that no row of
@@ -425,7 +448,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) smem_add_release(&sh->vcnt[cc], 1);
+      if (lane == 0) mbar_arrive(&sh->values[cc]);
       PROF_ADD(2)
     }
     PROF_OUT(32, 4)
@@ -443,14 +466,15 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     float m = -1e30f;
     bool alive = true;
 
-    // O <- signs * fwht(alpha * sum(p n) + beta * O) / 128, in place (columns 0 .. 127 of the accumulator)
+    // O <- signs * fwht(alpha * sum(p n) + beta * O) / 128, in place (columns 0 .. 127 of the accumulator).  The two warps of a group of
+    // rows share it: each takes two chunks of 32 columns for index bits 0 .. 4, then half of the column pairs for bits 5, 6.
     auto unrotate = [&]() {
       uint32_t r4[4];
       tc5::ld4(tl_ + TM_O + 128, r4);
       tc5::wait_ld();
       const float add = p.lut_alpha * __uint_as_float(r4[2]);
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {  // index bits 0 .. 4: inside each chunk of 32 columns
+      for (int c = 2 * hf; c < 2 * hf + 2; ++c) {
         uint32_t r[32];
         tc5::ld32(tl_ + TM_O + 32 * c, r);
         tc5::wait_ld();
@@ -469,9 +493,18 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
         tc5::st32(tl_ + TM_O + 32 * c, r);
       }
-      tc5::wait_st();
+      auto both = [&](uint32_t u) {  // the other warp's columns are written
+        tc5::wait_st();
+        tc5::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->rot[wq]);
+        const bool ok = warp_wait(&sh->rot[wq], u, p.status, 56);
+        tc5::fence_after();
+        return ok;
+      };
+      if (!both(0)) return false;
 #pragma unroll 1
-      for (int j0 = 0; j0 < 32; j0 += 8) {  // index bits 5, 6: across the four chunks
+      for (int j0 = 16 * hf; j0 < 16 * hf + 16; j0 += 8) {  // index bits 5, 6: across the four chunks
         uint32_t a0[8], a1[8], a2[8], a3[8];
         tc5::ld8(tl_ + TM_O + j0, a0);
         tc5::ld8(tl_ + TM_O + 32 + j0, a1);
@@ -492,7 +525,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         tc5::st8(tl_ + TM_O + 64 + j0, a2);
         tc5::st8(tl_ + TM_O + 96 + j0, a3);
       }
-      tc5::wait_st();
+      return both(1);
     };
     // 32 scores -> weights with the running maximum -> 16 columns of fp16 pairs
     auto weights32 = [&](const uint32_t (&r)[32], uint32_t tp, float negm) {
@@ -503,20 +536,6 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       tc5::st16(tp, pk);
     };
 
-    auto turn_is = [&](int u, int where) {  // half tiles 0 .. u-1 are settled; bounded
-      if (smem_load_acquire(&sh->turn[wq]) >= u) return true;
-      const long long t0 = clock64();
-      for (uint32_t spin = 1;; ++spin) {
-        if (smem_load_acquire(&sh->turn[wq]) >= u) return true;
-        if ((spin & 255u) == 0u) {
-          if (*reinterpret_cast<volatile int32_t*>(p.status) != 0) return false;
-          if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
-            if (lane == 0 && atomicCAS(p.status, 0, 1) == 0) p.status[1] = blockIdx.x, p.status[2] = where;
-            return false;
-          }
-        }
-      }
-    };
     PROF_DECL(8)
     for (int n = 0; n < NT && alive; ++n) {  // half tile u = (tile n, half hf): tokens 64 hf .. 64 hf + 63
       const int u = 2 * n + hf, e = n & 1;
@@ -532,13 +551,13 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       const int jw = MODE == MODE_SLIDING ? (int)max((int64_t)0, min((int64_t)64, pq - p.window + 1 - key0)) : 0;
       const int jl = (int)max((int64_t)0, min((int64_t)n_valid, rel));                    // keys [0, jl) of the half are visible to this row
       const uint32_t tS = tl_ + TM_S + 64 * hf, tP = tl_ + TM_P + 32 * hf;
-      if (hf == 0 && n == NP && NP > 0) {  // first window tile after pages: leave the rotated space of the value codec
+      if (n == NP && NP > 0) {  // first window tile after pages: leave the rotated space of the value codec
         if (!(warp_wait(&sh->odone[0], (uint32_t)(n - 1) & 1u, p.status, 46) && warp_wait(&sh->odone[1], (uint32_t)(n - 1) & 1u, p.status, 46))) {
           alive = false;
           break;
         }
         tc5::fence_after();
-        unrotate();
+        if (!unrotate()) { alive = false; break; }
       }
       PROF_ADD(0)
       if (!warp_wait(&sh->sdone[hf][e], (uint32_t)(n >> 1) & 1u, p.status, 47)) { alive = false; break; }
@@ -551,7 +570,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       tc5::wait_ld();
       tc5::fence_before();
       __syncwarp();
-      if (lane == 0) smem_add_release(&sh->scnt[hf], 1);
+      if (lane == 0) mbar_arrive(&sh->scores[hf]);
       PROF_ADD(2)
       if (masked) {
 #pragma unroll
@@ -566,7 +585,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
 #pragma unroll
       for (int i = 4; i < 32; ++i) t4[i & 3] = fmaxf(fmaxf(t4[i & 3], __uint_as_float(ra[i])), __uint_as_float(rb[i]));
       const float ts = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2;
-      if (!__all_sync(0xffffffffu, turn_is(u, 53))) { alive = false; break; }
+      // the half before: set 0 follows set 1's previous tile, set 1 follows set 0's same tile
+      if (u > 0 && !warp_wait(&sh->turn[hf ^ 1][wq], (uint32_t)(hf ? n : n - 1) & 1u, p.status, 53)) { alive = false; break; }
       if (u > 0) m = sh->m[row];
       // Lazy maximum: it moves only when a score exceeds it by more than 8 (weights stay below 2^8).  Then the whole warp (TMEM
       // access is warp-wide) rescales its rows of the accumulator once every earlier U3 has finished.
@@ -602,7 +622,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       // this half's maximum is settled: the other set may settle the next one
       sh->m[row] = m;
       __syncwarp();
-      if (lane == 0) smem_add_release(&sh->turn[wq], 1);
+      if (lane == 0) mbar_arrive(&sh->turn[hf][wq]);
       PROF_ADD(5)
       // the weight columns of this half still feed U3 of the previous tile's same half
       if (n >= 1 && !warp_wait(&sh->odone[hf], (uint32_t)(n - 1) & 1u, p.status, 48)) { alive = false; break; }
@@ -614,104 +634,75 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       tc5::wait_st();
       tc5::fence_before();
       __syncwarp();
-      if (lane == 0) smem_add_release(&sh->pcnt[hf], 1);
+      if (lane == 0) mbar_arrive(&sh->weights[hf]);
       PROF_ADD(4)
     }
     PROF_OUT(48, 8)
-    if (hf == 1) alive = false;  // the first set finishes the rows
+    // ---- the last U3, the rotation if no window tile undid it, normalise and store: each set takes 64 of the channels ----
     if (alive && NT > 0) {
-      alive = __all_sync(0xffffffffu, turn_is(2 * NT, 54));
+      alive = warp_wait(&sh->turn[1][wq], (uint32_t)(NT - 1) & 1u, p.status, 54);  // the last half is settled
       m = sh->m[row];
     }
-
-    // ---- the last U3, the rotation if no window tile undid it, normalise and store ----
     if (alive && NT > 0 && !(warp_wait(&sh->odone[0], (uint32_t)(NT - 1) & 1u, p.status, 49) && warp_wait(&sh->odone[1], (uint32_t)(NT - 1) & 1u, p.status, 49)))
       alive = false;
-    if (MODE == MODE_PREFIX && alive) {
-      // record of this share: accumulators as the value table's affine map leaves them (the rotation is undone where the parts are
-      // merged), running maximum, sum of weights
-      const bool live = row < PP * G && ip < n_members;
-      float* rec = p.part + (((int64_t)(live ? p.members[m0 + ip] : 0) * H + h * G + qi) * n_split + share) * PREFIX_PART_STRIDE;
-      float lsum = 0.f, add = 0.f;
-      if (NT > 0) {
-        tc5::fence_after();
-        uint32_t r4[4];
-        tc5::ld4(tl_ + TM_O + 128, r4);
-        tc5::wait_ld();
-        lsum = __uint_as_float(r4[0]) + __uint_as_float(r4[1]), add = p.lut_alpha * __uint_as_float(r4[2]);
-      }
-      // a row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used) and
-      // leave 512 bytes at a time (16 bytes of 32 rows per store kept the store unit busy for 2 us)
-      float* stage = reinterpret_cast<float*>(kop0) + (size_t)wq * 32 * PREFIX_PART_STRIDE;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        if (NT > 0) {
-          tc5::ld32(tl_ + TM_O + 32 * c, r);
-          tc5::wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(p.lut_beta, __uint_as_float(r[i]), add));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          reinterpret_cast<uint4*>(stage + lane * PREFIX_PART_STRIDE + 32 * c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-      }
-      __syncwarp();
-      const uint64_t rec_u = live ? reinterpret_cast<uint64_t>(rec) : 0;
+    float lsum = 0.f, add = 0.f;
+    if (alive && NT > 0) {
+      tc5::fence_after();
+      if (MODE != MODE_PREFIX && NW == 0) alive = unrotate();
+      uint32_t r4[4];
+      tc5::ld4(tl_ + TM_O + 128, r4);
+      tc5::wait_ld();
+      lsum = __uint_as_float(r4[0]) + __uint_as_float(r4[1]);
+      if (MODE == MODE_PREFIX) add = p.lut_alpha * __uint_as_float(r4[2]);
+    }
+    if (alive) {
+      // A row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used) and leave
+      // whole lines at a time.  (16 bytes of 32 rows per store kept the store unit busy for 2 us.)
+      uint4* stage = reinterpret_cast<uint4*>(kop0) + (warp - 8) * 32 * 17;
+      auto rows_out = [&](auto n16_, uint64_t to) {  // n16 16-byte pieces per row, row r to the address that lane r holds (0: nowhere)
+        constexpr int n16 = decltype(n16_)::value;
+        __syncwarp();
 #pragma unroll 4
-      for (int i = 0; i < 32; ++i) {
-        float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, rec_u, i));
-        if (dst) reinterpret_cast<float4*>(dst)[lane] = reinterpret_cast<const float4*>(stage + i * PREFIX_PART_STRIDE)[lane];
-      }
-      if (live) *reinterpret_cast<float4*>(rec + 128) = make_float4(NT > 0 ? m : -INFINITY, lsum, 0.f, 0.f);
-    } else if (alive) {
-      float inv = 0.f;
-      if (NT > 0) {
-        tc5::fence_after();
-        if (NW == 0) unrotate();
-        uint32_t r4[4];
-        tc5::ld4(tl_ + TM_O + 128, r4);
-        tc5::wait_ld();
-        const float l = __uint_as_float(r4[0]) + __uint_as_float(r4[1]);
-        inv = (l > 0.f) ? 1.f / l : 0.f;
-      }
-      const int64_t grow = ((int64_t)b * H + h * G + qi) * p.n_q + ip;  // row of q / out
-      if (n_split > 1) {  // partial record of this share: unnormalised accumulators, running maximum, sum of weights
-        float* rec = p.part + (grow * n_split + share) * PF_PART_STRIDE;
-        float lsum = 0.f;
-        if (NT > 0) {
-          uint32_t r4[4];
-          tc5::ld4(tl_ + TM_O + 128, r4);
-          tc5::wait_ld();
-          lsum = __uint_as_float(r4[0]) + __uint_as_float(r4[1]);
+        for (int i = 0; i < 32; i += 32 / n16) {
+          const int r = i + lane / n16;
+          uint4* dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, r));
+          if (dst) dst[lane % n16] = stage[r * (n16 + 1) + lane % n16];
         }
+      };
+      if (MODE == MODE_PREFIX || n_split > 1) {
+        // partial record of this share: unnormalised accumulators, running maximum, sum of weights.  MODE_PREFIX: accumulators as the value
+        // table's affine map leaves them, the rotation is undone where the parts are merged
+        constexpr int STRIDE = MODE == MODE_PREFIX ? PREFIX_PART_STRIDE : PF_PART_STRIDE;
+        const bool live = MODE == MODE_PREFIX ? (row < PP * G && ip < n_members) : ip < p.n_q;
+        int64_t grow = 0;
+        if (live) grow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+        float* rec = p.part + (grow * n_split + share) * STRIDE;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t r[32];
           if (NT > 0) {
-            tc5::ld32(tl_ + TM_O + 32 * c, r);
+            tc5::ld32(tl_ + TM_O + 64 * hf + 32 * c, r);
             tc5::wait_ld();
+            if (MODE == MODE_PREFIX) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(p.lut_beta, __uint_as_float(r[i]), add));
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = 0u;
           }
-          if (ip < p.n_q) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(rec + 32 * c)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-          }
+          for (int j = 0; j < 8; ++j) stage[lane * 17 + 8 * c + j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
         }
-        if (ip < p.n_q) *reinterpret_cast<float4*>(rec + 128) = make_float4(m, lsum, 0.f, 0.f);
+        rows_out(std::integral_constant<int, 16>{}, live ? reinterpret_cast<uint64_t>(rec + 64 * hf) : 0);
+        if (live && hf == 0) *reinterpret_cast<float4*>(rec + 128) = make_float4(MODE == MODE_PREFIX && NT == 0 ? -INFINITY : m, lsum, 0.f, 0.f);
       } else {
-        // through shared memory, as above: two rows of 256 bytes per store
-        uint4* stage = reinterpret_cast<uint4*>(kop0) + (size_t)wq * 32 * 17;
+        const float inv = (lsum > 0.f) ? 1.f / lsum : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t r[32];
           if (NT > 0) {
-            tc5::ld32(tl_ + TM_O + 32 * c, r);
+            tc5::ld32(tl_ + TM_O + 64 * hf + 32 * c, r);
             tc5::wait_ld();
           } else {
 #pragma unroll
@@ -723,127 +714,84 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w4[i] = pack_h2(__uint_as_float(r[8 * j + 2 * i]) * inv, __uint_as_float(r[8 * j + 2 * i + 1]) * inv);
-            stage[lane * 17 + 4 * c + j] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            stage[lane * 9 + 4 * c + j] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
         }
-        __syncwarp();
-        const int64_t mine = ip < p.n_q ? grow : -1;
-#pragma unroll 4
-        for (int i = 0; i < 32; i += 2) {
-          const int64_t to = __shfl_sync(0xffffffffu, mine, i + (lane >> 4));
-          if (to >= 0) reinterpret_cast<uint4*>(p.out + to * HEAD_DIM)[lane & 15] = stage[(i + (lane >> 4)) * 17 + (lane & 15)];
-        }
+        const int64_t grow = ((int64_t)b * H + h * G + qi) * p.n_q + ip;  // row of q / out
+        rows_out(std::integral_constant<int, 8>{}, ip < p.n_q ? reinterpret_cast<uint64_t>(p.out + grow * HEAD_DIM + 64 * hf) : 0);
       }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P5_REG_SERVICE));
-    // ===================== service warps: 16 copies + U1, 17 U2, 18 U3 (19 idle) =====================
-    // Tile n:  copy -> full[n % 3];  A: U1 -> low;  per half hf:  B: U2 -> sdone[hf][n & 1];  C: U3 -> odone[hf].
-    // A(n) needs the copy landed and K_low of tile n-1 read by every key warp; B(n, hf) the keys of tile n and the
-    // scores of the same half of tile n-1 read; C(n, hf) the weights of the half and the values of tile n; copy(n) the
-    // raw stage of tile n-3 consumed by the key and value warps.  A thread gets an MMA out every 100 - 200 cycles, far
-    // less than the tensor pipe takes: the three contractions are issued by three warps, each polling only the counters
-    // its own action needs.  A whole warp walks its state machine, one elected lane issues.
+    // ===================== service warps: 16 U1, 17 U2, 18 U3, 19 copies =====================
+    // Tile n:  copy -> full[n % 3];  U1 -> low;  U2 -> sdone[0 / 1][n & 1];  per half hf:  U3 -> odone[hf].
+    // U1(n) needs the copy landed and K_low of tile n-1 read by every key warp; U2(n) the keys of tile n and both halves' scores of tile
+    // n-1 read; U3(n, hf) the weights of the half and the values of tile n; copy(n) the raw stage of tile n-3 read by the key and value
+    // warps.  Each contraction has a warp that waits for its operands and nothing else; one elected lane issues.
     const bool el = elect_one_p5();
-    long long t_last = clock64();
-    uint32_t idle = 0;
-    bool ok = true;
-    // bounded polling: gives up (and says where) once nothing has moved for the wait limit, or another wait gave up
-    auto stalled = [&](bool progressed, int where) {
-      if (progressed) {
-        idle = 0;
-      } else if ((++idle & 255u) == 0u) {
-        if (idle == 256u) t_last = clock64();
-        if (clock64() - t_last > WAIT_LIMIT_CYCLES || *reinterpret_cast<volatile int32_t*>(p.status) != 0) {
-          if (el && atomicCAS(p.status, 0, 1) == 0) p.status[1] = blockIdx.x, p.status[2] = where;
-          return true;
-        }
-      }
-      return false;
-    };
     if (warp == 16) {
       constexpr uint32_t ID_U1 = tc5::idesc_f16_f16(128, 128);
       const uint64_t d_stage = tc5::smem_desc(smem_u32(stage0), 128, AB_SBO), d_b = tc5::smem_desc(smem_u32(bop), 128, AB_SBO);
-      int nP = min(NP, P5_STAGES), nA = 0, sP = nP % P5_STAGES, sA = 0;  // the prologue issued the first copies
-      uint32_t phA = 0;
-      int slot = (nP < NP) ? table[page_of(nP)] : 0;  // page slot of the next copy, fetched one copy ahead
-      while (ok && nA < NP) {
-        bool progressed = false;
-        const int kc0 = smem_load_acquire(&sh->kcnt[0]), kc1 = smem_load_acquire(&sh->kcnt[1]);
-        const int vc = min(smem_load_acquire(&sh->vcnt[0]), smem_load_acquire(&sh->vcnt[1]));
-        const int kl0 = smem_load_acquire(&sh->klcnt[0]), kl1 = smem_load_acquire(&sh->klcnt[1]);
-        auto kdone = [&](int t) { return t < 0 || ((t & 1) ? kc1 : kc0) >= 8 * ((t >> 1) + 1); };   // every key warp is through tile t
-        auto kldone = [&](int t) { return t < 0 || ((t & 1) ? kl1 : kl0) >= 8 * ((t >> 1) + 1); };  // ... holds K_low of tile t in registers
-        // ---- A ----
-        if (nA < nP && kldone(nA - 1) && mbar_test_wait(&sh->full[sA], phA)) {
-          tc5::fence_after();
-          const uint64_t da = d_stage + (uint64_t)(sA * (STAGE_BYTES >> 4));
-          if (el) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int n = 0; n < NP; ++n) {
+        if (!warp_wait(&sh->full[s], ph, p.status, 40)) break;
+        if (n >= 1 && !warp_wait(&sh->klow, (uint32_t)(n - 1) & 1u, p.status, 57)) break;
+        tc5::fence_after();
+        if (el) {
+          const uint64_t da = d_stage + (uint64_t)(s * (STAGE_BYTES >> 4));
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) tc5::mma_ss(tmem + TM_KL, da + 16 * ks, d_b + 16 * ks, ID_U1, ks > 0);
-            tc5::commit(smem_u32(&sh->low));
-          }
-          __syncwarp();
-          ++nA;
-          if (++sA == P5_STAGES) sA = 0, phA ^= 1u;
-          progressed = true;
+          for (int ks = 0; ks < KS; ++ks) tc5::mma_ss(tmem + TM_KL, da + 16 * ks, d_b + 16 * ks, ID_U1, ks > 0);
+          tc5::commit(smem_u32(&sh->low));
         }
-        // ---- copy ----
-        if (nP < NP && (nP < P5_STAGES || (kdone(nP - P5_STAGES) && vc >= 4 * (nP - P5_STAGES + 1)))) {
-          if (el) copy_tile(sP, slot);
-          __syncwarp();
-          ++nP;
-          if (++sP == P5_STAGES) sP = 0;
-          if (nP < NP) slot = table[page_of(nP)];
-          progressed = true;
-        }
-        if (stalled(progressed, 40)) ok = false;
+        __syncwarp();
+        if (++s == P5_STAGES) s = 0, ph ^= 1u;
       }
     } else if (warp == 17) {
       // one contraction per tile: the rows of Q are read from shared memory once for its 128 keys (twice per tile in halves of 64, which
       // made U2 wait for shared memory); each half's softmax warps have a barrier of their own
       constexpr uint32_t ID_U2 = tc5::idesc_f16_f32(128, 128);
       const uint64_t d_q = tc5::smem_desc(smem_u32(qop), 128, OP_SBO), d_k = tc5::smem_desc(smem_u32(kop0), 128, OP_SBO);
-      int n = 0;  // tiles issued
-      while (ok && n < NT) {
-        const int kc = smem_load_acquire(&sh->kcnt[n & 1]), sc = min(smem_load_acquire(&sh->scnt[0]), smem_load_acquire(&sh->scnt[1]));
-        bool progressed = false;
-        if (kc >= 8 * ((n >> 1) + 1) && sc >= 4 * n) {
-          tc5::fence_after();
+      for (int n = 0; n < NT; ++n) {
+        if (n >= 1 && !(warp_wait(&sh->scores[0], (uint32_t)(n - 1) & 1u, p.status, 51) && warp_wait(&sh->scores[1], (uint32_t)(n - 1) & 1u, p.status, 51))) break;
+        if (!warp_wait(&sh->keys[n & 1], (uint32_t)(n >> 1) & 1u, p.status, 58)) break;
+        tc5::fence_after();
+        if (el) {
           const uint64_t db = d_k + (uint64_t)((n & 1) * (OP_BYTES >> 4));
-          if (el) {
 #pragma unroll
-            for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S, d_q + 16 * ks, db + 16 * ks, ID_U2, ks > 0);  // 144 channels
-            tc5::commit(smem_u32(&sh->sdone[0][n & 1]));
-            tc5::commit(smem_u32(&sh->sdone[1][n & 1]));
-          }
-          __syncwarp();
-          ++n;
-          progressed = true;
+          for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S, d_q + 16 * ks, db + 16 * ks, ID_U2, ks > 0);  // 144 channels
+          tc5::commit(smem_u32(&sh->sdone[0][n & 1]));
+          tc5::commit(smem_u32(&sh->sdone[1][n & 1]));
         }
-        if (stalled(progressed, 51)) ok = false;
+        __syncwarp();
       }
     } else if (warp == 18) {
       constexpr uint32_t ID_U3 = tc5::idesc_f16_f32(128, VROWS);
       const uint64_t d_v = tc5::smem_desc(smem_u32(vop), 128, V_SBO);
-      int uC = 0;
-      while (ok && uC < 2 * NT) {
-        const int hf = uC & 1, n = uC >> 1;
-        const int pc = smem_load_acquire(&sh->pcnt[hf]), vc = smem_load_acquire(&sh->vcnt[hf]);
-        bool progressed = false;
-        if (pc >= 4 * (n + 1) && vc >= 4 * (n + 1)) {
-          tc5::fence_after();
-          if (el) {
+      for (int u = 0; u < 2 * NT; ++u) {
+        const int hf = u & 1, n = u >> 1;
+        if (!warp_wait(&sh->values[hf], (uint32_t)n & 1u, p.status, 52)) break;
+        if (!warp_wait(&sh->weights[hf], (uint32_t)n & 1u, p.status, 59)) break;
+        tc5::fence_after();
+        if (el) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)  // 64 tokens of the half: weight columns 32 hf .., token chunks 8 hf ..
-              tc5::mma_ts(tmem + TM_O, tmem + TM_P + 32 * hf + 8 * ks, d_v + 64 * hf + 16 * ks, ID_U3, (uC > 0 || ks > 0) ? 1u : 0u);
-            tc5::commit(smem_u32(&sh->odone[hf]));
-          }
-          __syncwarp();
-          ++uC;
-          progressed = true;
+          for (int ks = 0; ks < 4; ++ks)  // 64 tokens of the half: weight columns 32 hf .., token chunks 8 hf ..
+            tc5::mma_ts(tmem + TM_O, tmem + TM_P + 32 * hf + 8 * ks, d_v + 64 * hf + 16 * ks, ID_U3, (u > 0 || ks > 0) ? 1u : 0u);
+          tc5::commit(smem_u32(&sh->odone[hf]));
         }
-        if (stalled(progressed, 52)) ok = false;
+        __syncwarp();
+      }
+    } else {
+      // copies of the tiles behind the first ones, which the prologue issued; the page's slot is fetched one copy ahead
+      int s = 0, slot = (P5_STAGES < NP) ? table[page_of(P5_STAGES)] : 0;
+      uint32_t ph = 0;
+      for (int n = P5_STAGES; n < NP; ++n) {
+        const int next = (n + 1 < NP) ? table[page_of(n + 1)] : 0;
+        if (!warp_wait(&sh->empty[s], ph, p.status, 60)) break;
+        if (el) copy_tile(s, slot);
+        __syncwarp();
+        slot = next;
+        if (++s == P5_STAGES) s = 0, ph ^= 1u;
       }
     }
   }
@@ -851,7 +799,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   // ---- epilogue: every role ends here; the tensor memory goes back before the CTA leaves ----
   tc5::fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 17) {
     tc5::fence_after();
     tc5::dealloc(tmem, TM_COLS);
   }
