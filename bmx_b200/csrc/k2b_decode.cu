@@ -636,41 +636,24 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 // heads, so that a window row is read and widened once for the group (the kernel above reads it once per query head).  Against a variant
 // of that kernel, in a step of 128 sequences x 8 KV heads x 4 query heads with 4 prefix records each: 87 -> 35 us; 32 sequences with 18
 // records 26 -> 10 us; one sequence: the same time.
-//   scores   2 * GQ lanes per token, 64 / GQ channels each (64 query values per lane in registers); the GQ partial sums are reduced by
-//            halves: each step a lane keeps the sums of half of its queries and hands over the other half
+//   scores   mma.sync over 16 tokens and eight queries per warp; operands straight from global memory, the channels taken in an order
+//            in which a lane's eight are one 16-byte piece (the order of a contraction is free)
 //   values   thread = (channel octet, token group of 16), GQ x 8 accumulators; every row is loaded once
 //   records  warp = query head (and half of the records for GQ = 4), lane = four channels, all loads of four records in flight
 // ---------------------------------------------------------------------------------------------
 template <int WALK, int GQ>
-__global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_group_kernel(const K2bMergeParams p) {
-  constexpr int LPT = 2 * GQ, CH = 64 / GQ, TPP = MERGE_THREADS / LPT;  // lanes per token, channels per lane, tokens per pass
-  constexpr int NB = 4;                                                // passes whose loads are in flight together
+__global__ void __launch_bounds__(MERGE_THREADS, GQ == 4 ? 3 : 2) k2b_merge_group_kernel(const K2bMergeParams p) {
+  constexpr int NV = 4, NB = 4;  // value rows and records of a thread in flight together
   extern __shared__ __align__(16) float msm[];
   const K2bGeom g = p.g;
   const int G = g.n_q_groups, cap4 = (p.tail_cap + 3) & ~3;
-  float* sc = msm;                    // [GQ][cap4] window scores, then weights
-  float* red = sc + GQ * cap4;        // [8][GQ][128] window accumulators per warp
-  float* qs = red;                    // [GQ][128] scaled queries, before that
+  float* sc = msm;                       // [GQ][cap4] window scores, then weights
+  float* red = sc + GQ * cap4;           // [8][GQ][128] window accumulators per warp
   float* rec = red + 8 * GQ * HEAD_DIM;  // [4][32][4] accumulators of the second half of the records (GQ = 4)
   float* sm = rec + 4 * HEAD_DIM;        // [8] window maxima, [8] window sums, [4][2] states of the second half
   int* si = reinterpret_cast<int*>(sm + 24);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.x, b = bh / g.h_kv, h = bh % g.h_kv;
-
-  if (warp == 0) {
-    int pre = 0, tot = 0;
-    for (int i = lane; i < p.batch; i += 32) {
-      const int t = page_span<WALK>(p.walk, p.n_pages[i], i).tiles * g.h_kv;
-      tot += t;
-      if (i < b) pre += t;
-    }
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) pre += __shfl_xor_sync(0xffffffffu, pre, m), tot += __shfl_xor_sync(0xffffffffu, tot, m);
-    if (lane == 0) si[0] = pre, si[1] = tot;
-  }
-  for (int i = tid; i < GQ * HEAD_DIM; i += MERGE_THREADS)
-    qs[i] = i < G * HEAD_DIM ? __half2float(p.q[(int64_t)bh * G * HEAD_DIM + i]) * p.scale_log2 : 0.f;
-  __syncthreads();
 
   const int tl = p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
   const __half* kt = p.k_tail + (int64_t)bh * p.tail_cap * HEAD_DIM;
@@ -683,57 +666,37 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_group_kernel(const
   }
   auto shown = [&](int t) { return t < tl && (WALK != WALK_SLIDING || t < hid0 || t >= hid1); };
   {
-    const int l = tid % LPT, tp = tid / LPT;
-    float qr[GQ][CH];
+    const int gr = lane >> 2, t4 = lane & 3;
+    uint4 qf[4];
 #pragma unroll
-    for (int qi = 0; qi < GQ; ++qi)
+    for (int j = 0; j < 4; ++j)
+      qf[j] = gr < G ? reinterpret_cast<const uint4*>(p.q + ((int64_t)bh * G + gr) * HEAD_DIM)[t4 + 4 * j] : make_uint4(0u, 0u, 0u, 0u);
+    for (int t0 = 16 * warp; t0 < tl; t0 += 16 * 8) {
+      const int ta = t0 + gr, tb = ta + 8;
+      uint4 ka[4], kb[4];
 #pragma unroll
-      for (int k = 0; k < CH; ++k) qr[qi][k] = qs[qi * HEAD_DIM + 64 * (k / 8) + 8 * l + k % 8];  // chunks l and, with 16 channels, 8 + l
-    for (int t0 = 0; t0 < tl; t0 += NB * TPP) {
-      uint4 kv[NB][CH / 8];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int t = t0 + i * TPP + tp;
-#pragma unroll
-        for (int c = 0; c < CH / 8; ++c)
-          kv[i][c] = shown(t) ? reinterpret_cast<const uint4*>(kt + (int64_t)t * HEAD_DIM)[l + 8 * c] : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < 4; ++j) {
+        ka[j] = shown(ta) ? reinterpret_cast<const uint4*>(kt + (int64_t)ta * HEAD_DIM)[t4 + 4 * j] : make_uint4(0u, 0u, 0u, 0u);
+        kb[j] = shown(tb) ? reinterpret_cast<const uint4*>(kt + (int64_t)tb * HEAD_DIM)[t4 + 4 * j] : make_uint4(0u, 0u, 0u, 0u);
       }
+      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        float d[GQ];
-#pragma unroll
-        for (int qi = 0; qi < GQ; ++qi) d[qi] = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH / 8; ++c) {
-          const uint32_t w[4] = {kv[i][c].x, kv[i][c].y, kv[i][c].z, kv[i][c].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(u32_as_h2(w[k]));
-#pragma unroll
-            for (int qi = 0; qi < GQ; ++qi) d[qi] = fmaf(f.y, qr[qi][8 * c + 2 * k + 1], fmaf(f.x, qr[qi][8 * c + 2 * k], d[qi]));
-          }
-        }
-#pragma unroll
-        for (int m = GQ / 2; m >= 1; m >>= 1) {
-          const bool up = (l & m) != 0;
-#pragma unroll
-          for (int k = 0; k < m; ++k) {
-            const float mine = up ? d[m + k] : d[k], other = up ? d[k] : d[m + k];
-            d[k] = mine + __shfl_xor_sync(0xffffffffu, other, m);
-          }
-        }
-        d[0] += __shfl_xor_sync(0xffffffffu, d[0], GQ);
-        const int t = t0 + i * TPP + tp;
-        if (l < GQ && t < tl) sc[l * cap4 + t] = shown(t) ? d[0] : -INFINITY;  // lane l ends with query l
+      for (int j = 0; j < 4; ++j) {
+        mma_f32acc(s0, s1, s2, s3, ka[j].x, kb[j].x, ka[j].y, kb[j].y, qf[j].x, qf[j].y);
+        mma_f32acc(s0, s1, s2, s3, ka[j].z, kb[j].z, ka[j].w, kb[j].w, qf[j].z, qf[j].w);
+      }
+      if (2 * t4 < GQ) {
+        if (ta < tl) sc[2 * t4 * cap4 + ta] = shown(ta) ? s0 * p.scale_log2 : -INFINITY, sc[(2 * t4 + 1) * cap4 + ta] = shown(ta) ? s1 * p.scale_log2 : -INFINITY;
+        if (tb < tl) sc[2 * t4 * cap4 + tb] = shown(tb) ? s2 * p.scale_log2 : -INFINITY, sc[(2 * t4 + 1) * cap4 + tb] = shown(tb) ? s3 * p.scale_log2 : -INFINITY;
       }
     }
   }
   // ---- values: the first rows travel during the softmax ----
   const int c8 = tid & 15, tg = tid >> 4;
-  uint4 vv[NB];
+  uint4 vv[NV];
   auto load_values = [&](int t0) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < NV; ++i) {
       const int t = t0 + tg + 16 * i;
       vv[i] = shown(t) ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -753,6 +716,17 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_group_kernel(const
     for (int m = 16; m >= 1; m >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, m);
     if (lane == 0) sm[warp] = mx, sm[8 + warp] = ls;
   }
+  if (warp == 7) {  // tiles in front of this sequence and in all: which CTAs of the page-streaming kernel left records of it
+    int pre = 0, tot = 0;
+    for (int i = lane; i < p.batch; i += 32) {
+      const int t = page_span<WALK>(p.walk, p.n_pages[i], i).tiles * g.h_kv;
+      tot += t;
+      if (i < b) pre += t;
+    }
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) pre += __shfl_xor_sync(0xffffffffu, pre, m), tot += __shfl_xor_sync(0xffffffffu, tot, m);
+    if (lane == 0) si[0] = pre, si[1] = tot;
+  }
   __syncthreads();
   {
     float a[GQ][8];
@@ -760,10 +734,10 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_group_kernel(const
     for (int qi = 0; qi < GQ; ++qi)
 #pragma unroll
       for (int k = 0; k < 8; ++k) a[qi][k] = 0.f;
-    for (int t0 = 0; t0 < tl; t0 += 16 * NB) {
+    for (int t0 = 0; t0 < tl; t0 += 16 * NV) {
       if (t0 > 0) load_values(t0);
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < NV; ++i) {
         const int t = t0 + tg + 16 * i;
         const uint32_t w[4] = {vv[i].x, vv[i].y, vv[i].z, vv[i].w};
         float f[8];
@@ -949,8 +923,14 @@ static int launch_merge_group(const K2bMergeParams& mp, size_t smem, cudaStream_
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
   const int G = mp.g.n_q_groups, gq = G <= 4 ? 4 : 8;
   if (walk != WALK_ALL) {
-    const size_t gsmem = ((size_t)gq * ((mp.tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
+    size_t gsmem = ((size_t)gq * ((mp.tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
     BMXK_REQUIRE(gsmem <= GROUP_MERGE_SMEM, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
+    // While the page-streaming kernel drains, the blocks would pile up three to an SM on the SMs that are free already; a block that asks for
+    // more shared memory keeps them apart as long as the grid is small enough to spread (256 pairs: 63 -> 60 us a step; 128 pairs 52 -> 47).
+    // The blocks of eight query heads are two to an SM by their registers; one to an SM starts too late (126 pairs: 37 -> 41 us).
+    const int pairs = mp.batch * mp.g.h_kv, per_sm = pairs <= num_sms() && gq == 4 ? 1 : pairs <= 2 * num_sms() ? 2 : 3;
+    const size_t spread = per_sm == 1 ? 120 * 1024 : per_sm == 2 ? 80 * 1024 : 0;
+    if (gsmem < spread) gsmem = spread;
     if (walk == WALK_OWN) return gq == 4 ? launch_merge_group<WALK_OWN, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_OWN, 8>(mp, gsmem, s, after_main);
     return gq == 4 ? launch_merge_group<WALK_SLIDING, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_SLIDING, 8>(mp, gsmem, s, after_main);
   }

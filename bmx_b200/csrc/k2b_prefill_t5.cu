@@ -463,6 +463,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     const uint32_t tl_ = tmem + ((uint32_t)(32 * wq) << 16);
     const int qi = MODE == MODE_PREFIX ? row % G : row / PP, ip = MODE == MODE_PREFIX ? i0 + row / G : i0 + row % PP;
     const int64_t pq = p.q_pos0 + ip;
+    const bool in_group = MODE == MODE_PREFIX && row < PP * G && ip < n_members;
+    const int my_seq = in_group ? p.members[m0 + ip] : 0;  // for the record at the end
     float m = -1e30f;
     bool alive = true;
 
@@ -673,9 +675,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         // partial record of this share: unnormalised accumulators, running maximum, sum of weights.  MODE_PREFIX: accumulators as the value
         // table's affine map leaves them, the rotation is undone where the parts are merged
         constexpr int STRIDE = MODE == MODE_PREFIX ? PREFIX_PART_STRIDE : PF_PART_STRIDE;
-        const bool live = MODE == MODE_PREFIX ? (row < PP * G && ip < n_members) : ip < p.n_q;
-        int64_t grow = 0;
-        if (live) grow = MODE == MODE_PREFIX ? (int64_t)p.members[m0 + ip] * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+        const bool live = MODE == MODE_PREFIX ? in_group : ip < p.n_q;
+        const int64_t grow = MODE == MODE_PREFIX ? (int64_t)my_seq * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
         float* rec = p.part + (grow * n_split + share) * STRIDE;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
