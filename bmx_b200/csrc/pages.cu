@@ -125,25 +125,31 @@ extern "C" int bmxk_copy_slots(int n_arrays, const void* const* src, void* const
   free(seen);
   BMXK_REQUIRE(why == nullptr, "bmxk_copy_slots: pair %d (%d -> %d): %s", at, src_slots[at], dst_slots[at], why);
 
-  // Small calls (a fork) carry few parameters; 3000 pairs are 24 KB of the 32 KB a launch may carry.
+  // A launch carries as many pairs as its parameters have room for (32 KB at most); small calls (a fork) carry few, and in between the
+  // parameters of 3000 pairs would take the device longer to fetch than those of 1000.
   auto fill = [&](auto& p) {
     memcpy(p.a, arr, sizeof(arr));
     p.n_arrays = n_arrays, p.chunks = (int)chunks;
   };
   const int most = (int)((1LL << 30) / chunks);  // blocks of one launch
   for (int i = 0; i < n;) {
-    if (n - i <= 64 && n - i <= most) {
+    const int m = n - i < most ? n - i : most;
+    int rc, done;
+    if (m <= 64) {
       CopyParams<64> p;
       fill(p);
-      return launch_copy(p, src_slots + i, dst_slots + i, n - i, (cudaStream_t)stream);
+      done = m, rc = launch_copy(p, src_slots + i, dst_slots + i, done, (cudaStream_t)stream);
+    } else if (m <= 1000) {
+      CopyParams<1000> p;
+      fill(p);
+      done = m, rc = launch_copy(p, src_slots + i, dst_slots + i, done, (cudaStream_t)stream);
+    } else {
+      CopyParams<3000> p;
+      fill(p);
+      done = m < 3000 ? m : 3000, rc = launch_copy(p, src_slots + i, dst_slots + i, done, (cudaStream_t)stream);
     }
-    CopyParams<3000> p;
-    fill(p);
-    int m = n - i < 3000 ? n - i : 3000;
-    if (m > most) m = most;
-    const int rc = launch_copy(p, src_slots + i, dst_slots + i, m, (cudaStream_t)stream);
     if (rc) return rc;
-    i += m;
+    i += done;
   }
   return BMXK_OK;
 }

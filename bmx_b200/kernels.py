@@ -10,6 +10,7 @@ import array
 import contextlib
 import ctypes
 import functools
+import itertools
 import struct
 
 import torch
@@ -375,9 +376,10 @@ def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_page
     g = pool.geom
     h_kv, batch, half, i32 = g.h_kv, q.shape[0], torch.float16, torch.int32
     assert q.dtype is half and q.is_contiguous() and q.shape[1] == h_kv * g.n_q_groups and q.shape[-1] == HEAD_DIM
-    assert page_table.dtype is i32 and page_table.dim() == 2 and page_table.shape[0] == batch and page_table.stride(1) == 1
-    assert n_pages.dtype is i32 and n_pages.dim() == 1 and n_pages.numel() == batch and n_pages.is_contiguous()
-    assert 0 <= max_pages <= page_table.shape[1], f"max_pages={max_pages}: the page table has {page_table.shape[1]} columns"
+    rows, columns = page_table.shape
+    assert page_table.dtype is i32 and rows == batch and page_table.stride(1) == 1
+    assert n_pages.dtype is i32 and n_pages.shape == (batch,) and n_pages.is_contiguous()
+    assert 0 <= max_pages <= columns, f"max_pages={max_pages}: the page table has {columns} columns"
     assert signs.dtype is torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
     if max_pages > 0:
         assert basis_f16.dtype is half and basis_f16.is_contiguous() and basis_f16.numel() == h_kv * HEAD_DIM * g.rank
@@ -388,14 +390,14 @@ def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_page
         return 0
     shape = k_tail.shape
     assert k_tail.dtype is half and v_tail.dtype is half and k_tail.is_contiguous() and v_tail.is_contiguous()
-    assert len(shape) == 4 and shape[0] == batch and shape[1] == h_kv and shape[3] == HEAD_DIM and v_tail.shape == shape
-    assert tail_len.dtype is i32 and tail_len.dim() == 1 and tail_len.numel() == batch and tail_len.is_contiguous()
+    assert shape == (batch, h_kv, shape[2], HEAD_DIM) and v_tail.shape == shape
+    assert tail_len.dtype is i32 and tail_len.shape == (batch,) and tail_len.is_contiguous()
     return shape[2]
 
 
 def _check_out(out: torch.Tensor | None, q: torch.Tensor, dtypes: tuple) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=torch.float16, device=q.device)
+        return torch.empty_like(q)
     _require_device_visible(out)
     assert out.dtype in dtypes and out.is_contiguous() and out.shape == q.shape
     return out
@@ -666,12 +668,13 @@ def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
     n, n_src, n_dst = len(srcs), srcs[0].shape[0], dsts[0].shape[0]
     sizes = []
     for s, d in zip(srcs, dsts):
-        if s.dtype != d.dtype or s.dim() < 2 or s.shape[1:] != d.shape[1:]:
+        if s.dim() < 2 or d is not s and (s.dtype != d.dtype or s.shape[1:] != d.shape[1:]):
             raise ValueError(f"copy_slots: {tuple(s.shape)} {s.dtype} cannot be copied to {tuple(d.shape)} {d.dtype}")
         if s.shape[0] != n_src or d.shape[0] != n_dst:
             raise ValueError("copy_slots: arrays of one call have the same number of slots")
         size, src_stride = _slot_bytes(s)
-        sizes.append((s.data_ptr(), d.data_ptr(), src_stride, src_stride if d is s else _slot_bytes(d)[1], size))
+        at = s.data_ptr()
+        sizes.append((at, at, src_stride, src_stride, size) if d is s else (at, d.data_ptr(), src_stride, _slot_bytes(d)[1], size))
     a, a_at, a_n = _slot_list(src_slots)
     b, b_at, b_n = _slot_list(dst_slots)
     if a_n != b_n:
@@ -679,9 +682,9 @@ def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
     if a_n == 0:
         return
     # the five host arrays of the call in one block of 64-bit words: sources, destinations, their strides, sizes
-    words = array.array("q", [x[k] for k in range(5) for x in sizes])
+    words = array.array("q", itertools.chain.from_iterable(zip(*sizes)))
     at = words.buffer_info()[0]
-    with _on_device_of(*srcs, *dsts):
+    with _on_device_of(*srcs, *(() if dsts is srcs else dsts)):
         call("bmxk_copy_slots", n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, a_at, b_at, a_n, n_src, n_dst, _stream())
 
 
