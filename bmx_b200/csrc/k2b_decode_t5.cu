@@ -533,17 +533,15 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
           // the page-table entry of this tile, for the copy warp: a global load there would sit in front of every
           // release it does, so it is fetched here, where loads are prefetched anyway
           const int slot = p.page_table[(int64_t)b * p.table_stride + j];
-          float cs[2], sn[2], x1[2][GQ], x2[2][GQ];
+          // lane = rotary pairs (c, c + 64) and (c + 1, c + 65), c = 2 * lane: adjacent channels on both sides, one word per load and store
+          uint32_t x1[GQ], x2[GQ];
+          const uint32_t csw = reinterpret_cast<const uint32_t*>(p.rope_cos + t0 * HEAD_DIM)[lane];
+          const uint32_t snw = reinterpret_cast<const uint32_t*>(p.rope_sin + t0 * HEAD_DIM)[lane];
 #pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int c = lane + 32 * jj;  // rotary pair (c, c + 64)
-            cs[jj] = __half2float(p.rope_cos[t0 * HEAD_DIM + c]);
-            sn[jj] = __half2float(p.rope_sin[t0 * HEAD_DIM + c]);
-#pragma unroll
-            for (int qi = 0; qi < GQ; ++qi) {
-              x1[jj][qi] = (qi < G) ? __half2float(qsrc[qi * HEAD_DIM + c]) : 0.f;
-              x2[jj][qi] = (qi < G) ? __half2float(qsrc[qi * HEAD_DIM + c + 64]) : 0.f;
-            }
+          for (int qi = 0; qi < GQ; ++qi) {
+            const uint32_t* qw = reinterpret_cast<const uint32_t*>(qsrc + qi * HEAD_DIM);
+            x1[qi] = (qi < G) ? qw[lane] : 0u;
+            x2[qi] = (qi < G) ? qw[lane + 32] : 0u;
           }
           if (lane == 0) {
             sh->slot_ring[w.it & 15] = slot;
@@ -551,16 +549,16 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
           }
           if (!wait_or_flag(&sh->empty[s], ph, p.status, 3)) { alive = false; break; }
           __half* qr = reinterpret_cast<__half*>(qb0 + (size_t)s * T5_QB_BYTES);
-#pragma unroll
-          for (int jj = 0; jj < 2; ++jj) {
-            const int c = lane + 32 * jj;
-            const int k1 = 32 * (c >> 4) + (c & 15), k2 = k1 + 16;
+          {
+            const int c = 2 * lane, k1 = 32 * (c >> 4) + (c & 15), k2 = k1 + 16;
+            const float2 cs = __half22float2(u32_as_h2(csw)), sn = __half22float2(u32_as_h2(snw));
 #pragma unroll
             for (int qi = 0; qi < GQ; ++qi)
               if (qi < G) {
-                const float a = x1[jj][qi] * p.scale_log2, bb = x2[jj][qi] * p.scale_log2;
-                qr[(k1 >> 3) * 64 + qi * 8 + (k1 & 7)] = __float2half_rn(a * cs[jj] + bb * sn[jj]);
-                qr[(k2 >> 3) * 64 + qi * 8 + (k2 & 7)] = __float2half_rn(bb * cs[jj] - a * sn[jj]);
+                const float2 f1 = __half22float2(u32_as_h2(x1[qi])), f2 = __half22float2(u32_as_h2(x2[qi]));
+                const float a0 = f1.x * p.scale_log2, b0 = f2.x * p.scale_log2, a1 = f1.y * p.scale_log2, b1 = f2.y * p.scale_log2;
+                *reinterpret_cast<__half2*>(qr + (k1 >> 3) * 64 + qi * 8 + (k1 & 7)) = __floats2half2_rn(a0 * cs.x + b0 * sn.x, a1 * cs.y + b1 * sn.y);
+                *reinterpret_cast<__half2*>(qr + (k2 >> 3) * 64 + qi * 8 + (k2 & 7)) = __floats2half2_rn(b0 * cs.x - a0 * sn.x, b1 * cs.y - a1 * sn.y);
               }
           }
           if (new_seg) {
