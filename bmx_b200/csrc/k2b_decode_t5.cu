@@ -149,6 +149,33 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
     }
   }
 
+  // What the rotation warps need of a tile; in the short walks that of the first two tiles is requested here, ahead of the prologue (a
+  // load of memory that the SM has not touched takes 1 - 3 us, and the first tile is most of such a walk).
+  int slot = 0;
+  uint32_t csw = 0, snw = 0, x1[GQ], x2[GQ];
+  auto load_tile = [&](const TileCursor& cur) {
+    const int b = cur.b, h = cur.h, j = page_of(b, cur.j);
+    const int64_t t0 = p.pos_offset + (int64_t)j * TILE_TOKENS;
+    const __half* qsrc = p.q + ((int64_t)b * g.h_kv + h) * G * HEAD_DIM;
+    // the page-table entry of this tile, for the copy warp: a global load there would sit in front of every
+    // release it does, so it is fetched here, where loads are prefetched anyway
+    slot = p.page_table[(int64_t)b * p.table_stride + j];
+    // lane = rotary pairs (c, c + 64) and (c + 1, c + 65), c = 2 * lane: adjacent channels on both sides, one word per load and store
+    csw = reinterpret_cast<const uint32_t*>(p.rope_cos + t0 * HEAD_DIM)[lane];
+    snw = reinterpret_cast<const uint32_t*>(p.rope_sin + t0 * HEAD_DIM)[lane];
+#pragma unroll
+    for (int qi = 0; qi < GQ; ++qi) {
+      const uint32_t* qw = reinterpret_cast<const uint32_t*>(qsrc + qi * HEAD_DIM);
+      x1[qi] = (qi < G) ? qw[lane] : 0u;
+      x2[qi] = (qi < G) ? qw[lane + 32] : 0u;
+    }
+  };
+  if (WALK != WALK_ALL && warp >= 26) {
+    TileCursor first = w.cur;
+    if (warp == 27 && n_tiles > 1) first.next(npg_sm, g.h_kv, 128, p.batch);
+    if (warp == 26 || n_tiles > 1) load_tile(first);
+  }
+
   // ---- prologue: zeroed operand rows, barriers, tensor memory ----
   for (int i = tid; i < (T5_STAGES + 2) * T5_QB_BYTES / 16; i += T5_THREADS) {
     uint8_t* base = (i < T5_STAGES * T5_QB_BYTES / 16) ? qb0 + (size_t)i * 16 : pbuf0 + ((size_t)i - T5_STAGES * T5_QB_BYTES / 16) * 16;
@@ -527,22 +554,8 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
         const bool new_seg = (w.seg != prev_seg);
         if (new_seg) first_prev = first_cur, first_cur = w.it, prev_seg = w.seg;
         if ((w.it & 1) == rw) {
-          const int b = w.cur.b, h = w.cur.h, j = page_of(b, w.cur.j);
-          const int64_t t0 = p.pos_offset + (int64_t)j * TILE_TOKENS;
-          const __half* qsrc = p.q + ((int64_t)b * g.h_kv + h) * G * HEAD_DIM;
-          // the page-table entry of this tile, for the copy warp: a global load there would sit in front of every
-          // release it does, so it is fetched here, where loads are prefetched anyway
-          const int slot = p.page_table[(int64_t)b * p.table_stride + j];
-          // lane = rotary pairs (c, c + 64) and (c + 1, c + 65), c = 2 * lane: adjacent channels on both sides, one word per load and store
-          uint32_t x1[GQ], x2[GQ];
-          const uint32_t csw = reinterpret_cast<const uint32_t*>(p.rope_cos + t0 * HEAD_DIM)[lane];
-          const uint32_t snw = reinterpret_cast<const uint32_t*>(p.rope_sin + t0 * HEAD_DIM)[lane];
-#pragma unroll
-          for (int qi = 0; qi < GQ; ++qi) {
-            const uint32_t* qw = reinterpret_cast<const uint32_t*>(qsrc + qi * HEAD_DIM);
-            x1[qi] = (qi < G) ? qw[lane] : 0u;
-            x2[qi] = (qi < G) ? qw[lane + 32] : 0u;
-          }
+          const int h = w.cur.h;
+          if (WALK == WALK_ALL || w.it != rw) load_tile(w.cur);
           if (lane == 0) {
             sh->slot_ring[w.it & 15] = slot;
             asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(&sh->slot_seq[rw])), "r"(w.it + 1) : "memory");
