@@ -212,14 +212,26 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
     const __half2 c16th = __floats2half2_rn(0.0625f, 0.0625f);
     const __half2 cm72 = __floats2half2_rn(-72.f, -72.f);
     // rotation by this token's offset inside the tile, for rotary pairs 16k .. 16k+15 of both chunks
+    // (16 bytes at a time where the tables allow it: every load of a warp touches 32 rows, and word by word the 256 of them kept the load unit
+    // busy for the first 4 us)
     uint32_t cs_[2][8], sn_[2][8];
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.rope_cos) | reinterpret_cast<uintptr_t>(p.rope_sin)) & 15) == 0;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk) {
+      const __half* pc = p.rope_cos + (int64_t)row * HEAD_DIM + 16 * (k0 + kk);
+      const __half* ps = p.rope_sin + (int64_t)row * HEAD_DIM + 16 * (k0 + kk);
+      if (wide) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        cs_[kk][i] = *reinterpret_cast<const uint32_t*>(p.rope_cos + (int64_t)row * HEAD_DIM + 16 * (k0 + kk) + 2 * i);
-        sn_[kk][i] = *reinterpret_cast<const uint32_t*>(p.rope_sin + (int64_t)row * HEAD_DIM + 16 * (k0 + kk) + 2 * i);
+        for (int i = 0; i < 2; ++i) {
+          const uint4 c4 = reinterpret_cast<const uint4*>(pc)[i], s4 = reinterpret_cast<const uint4*>(ps)[i];
+          cs_[kk][4 * i] = c4.x, cs_[kk][4 * i + 1] = c4.y, cs_[kk][4 * i + 2] = c4.z, cs_[kk][4 * i + 3] = c4.w;
+          sn_[kk][4 * i] = s4.x, sn_[kk][4 * i + 1] = s4.y, sn_[kk][4 * i + 2] = s4.z, sn_[kk][4 * i + 3] = s4.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) cs_[kk][i] = reinterpret_cast<const uint32_t*>(pc)[i], sn_[kk][i] = reinterpret_cast<const uint32_t*>(ps)[i];
       }
+    }
     int s = 0;
     uint32_t fp = 0;
     for (int n = 0; n < n_tiles; ++n) {
