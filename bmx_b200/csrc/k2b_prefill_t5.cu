@@ -475,7 +475,12 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     const int wq = warp & 3, row = 32 * wq + lane, hf = (warp - 8) >> 2;
     const uint32_t tl_ = tmem + ((uint32_t)(32 * wq) << 16);
     const int qi = MODE == MODE_PREFIX ? row % G : row / PP, ip = MODE == MODE_PREFIX ? i0 + row / G : i0 + row % PP;
+    // positions relative to page_pos0: of this row and the CTA's first row, plus one; of the first key in this row's window and in the last row's
     const int64_t pq = p.q_pos0 + ip;
+    auto rel32 = [](int64_t x) { return (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, x)); };
+    const int row_rel = rel32(pq - page_pos0 + 1), first_rel = rel32(pq_min - page_pos0 + 1);
+    const int win_row = MODE == MODE_SLIDING ? rel32(pq - p.window + 1 - page_pos0) : 0, win_max = MODE == MODE_SLIDING ? rel32(lo_max - page_pos0) : 0;
+    const int sinks_rel = MODE == MODE_SLIDING ? rel32(p.sinks - page_pos0) : 0;
     const bool in_group = MODE == MODE_PREFIX && row < PP * G && ip < n_members;
     const int my_seq = in_group ? p.members[m0 + ip] : 0;  // for the record at the end
     float m = -1e30f;
@@ -554,17 +559,14 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     PROF_DECL(8)
     for (int n = 0; n < NT && alive; ++n) {  // half tile u = (tile n, half hf): tokens 64 hf .. 64 hf + 63
       const int u = 2 * n + hf, e = n & 1;
-      // keys of the half visible to this row / to the CTA's first row: position - first key position + 1
-      const int64_t key0 = (n < NP ? (MODE == MODE_SLIDING ? p.pos_offset + (int64_t)page_of(n) * 128 : page_pos0 + (int64_t)n * 128)
-                                   : tail_pos0 + (int64_t)(n - NP) * 128) + 64 * hf;
-      const int64_t rel = pq - key0 + 1, rel_min = pq_min - key0 + 1;
+      // Everything relative to the first key of the half (32 bits: a context is shorter than 2^31 tokens).  Keys [0, jl) of the half are at positions
+      // up to this row's; MODE_SLIDING: of those it sees [0, js) as sinks and [jw, jl) as its window.
+      const int from = (n < NP ? (MODE == MODE_SLIDING ? page_of(n) - T0 : n) : n_pg - T0 + (n - NP)) * 128 + 64 * hf;  // behind page_pos0
       const int n_valid = (n < NP) ? 64 : max(0, min(64, tl - (n - NP) * 128 - 64 * hf));
-      const bool masked = MODE != MODE_PREFIX && ((rel_min < 64) || (n_valid < 64) ||
-                                                  (MODE == MODE_SLIDING && key0 < lo_max && key0 + 64 > p.sinks));  // the same for the whole CTA
-      // MODE_SLIDING: of the half's keys this row sees [0, js) as sinks and [jw, jl) as its window
-      const int js = MODE == MODE_SLIDING ? (int)max((int64_t)0, min((int64_t)64, p.sinks - key0)) : 0;
-      const int jw = MODE == MODE_SLIDING ? (int)max((int64_t)0, min((int64_t)64, pq - p.window + 1 - key0)) : 0;
-      const int jl = (int)max((int64_t)0, min((int64_t)n_valid, rel));                    // keys [0, jl) of the half are visible to this row
+      const bool masked = MODE != MODE_PREFIX && (first_rel - from < 64 || n_valid < 64 ||
+                                                  (MODE == MODE_SLIDING && from < win_max && from + 64 > sinks_rel));  // the same for the whole CTA
+      const int jl = max(0, min(n_valid, row_rel - from));
+      const int js = MODE == MODE_SLIDING ? sinks_rel - from : 0, jw = MODE == MODE_SLIDING ? win_row - from : 0;
       const uint32_t tS = tl_ + TM_S + 64 * hf, tP = tl_ + TM_P + 32 * hf;
       if (n == NP && NP > 0) {  // first window tile after pages: leave the rotated space of the value codec
         if (!(warp_wait(&sh->odone[0], (uint32_t)(n - 1) & 1u, p.status, 46) && warp_wait(&sh->odone[1], (uint32_t)(n - 1) & 1u, p.status, 46))) {
