@@ -529,7 +529,8 @@ static int prefill_impl(const bmxk_k2b_geom* g, const void* q, int n_q, int64_t 
   if (!t5) rope_pages = 0;
   prm.n_split = n_split, prm.part = (float*)workspace;
   const size_t part_bytes = bmxk_k2b_prefill_workspace_bytes(g, n_q, batch, n_split), need = part_bytes + (sliding ? 0 : bmxk_k2b_prefill_rope_bytes(rope_pages));
-  prm.window = sliding ? sliding->window : 0, prm.sinks = sliding ? sliding->sinks : 0;
+  prm.window = sliding ? (int)(sliding->window < (1 << 30) ? sliding->window : 1 << 30) : 0;
+  prm.sinks = sliding ? (int)(sliding->sinks < (1 << 30) ? sliding->sinks : 1 << 30) : 0;
   prm.rope_pages = rope_pages, prm.rope_frag = sliding ? (uint4*)sliding->rope_frag : rope_pages > 0 ? reinterpret_cast<uint4*>((uint8_t*)workspace + part_bytes) : nullptr;
   BMXK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "bmxk_k2b_prefill_split: workspace of %zu bytes needed (16-byte aligned), %zu given", need, workspace_bytes);

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   constexpr uint32_t AB_SBO = RANK * 16;  // bytes between 8-row groups of the coef / basis operands
   extern __shared__ __align__(128) uint8_t smem[];
   const K2bGeom g = p.g;
-  const int G = g.n_q_groups, PP = 128 / G;  // query positions per CTA
+  const int G = g.n_q_groups, PP = p.pp;  // query heads per KV head; query positions (MODE_PREFIX: sequences) per CTA
   const int PB = k2b_page_block_bytes(128, g.group);
   const int STAGE_BYTES = COEF_BYTES + PB;
 
@@ -130,9 +130,14 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // the latest positions see the most pages: their blocks are scheduled first, so that the last wave is the lightest
   // (blockIdx.x = position block * n_split + share: the shares of a block run side by side)
-  const int n_split = p.n_split, share = (int)blockIdx.x % n_split, n_blocks = (int)gridDim.x / n_split;
-  const int b = blockIdx.z, h = blockIdx.y, i0 = (n_blocks - 1 - (int)blockIdx.x / n_split) * PP;
+  const int n_split = p.n_split, n_blocks = n_split == 1 ? (int)gridDim.x : (int)(gridDim.x / (unsigned)n_split);
+  const int block = n_split == 1 ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)n_split), share = (int)blockIdx.x - block * n_split;
+  const int b = blockIdx.z, h = blockIdx.y, i0 = (n_blocks - 1 - block) * PP;
   const int H = g.h_kv * G;
+  // Row m of the CTA: a query head and a position (MODE_PREFIX: a member of the group, any G up to 8, 128 - PP * G rows idle).  No divisions and
+  // no 64-bit arithmetic in what every thread runs here: it was half of the time to the first tile.
+  auto head_of = [&](int m) { return MODE == MODE_PREFIX ? m - (int)((uint32_t)(m * p.g_inv) >> 10) * G : m >> p.pp_log; };
+  auto pos_of = [&](int m) { return MODE == MODE_PREFIX ? (int)((uint32_t)(m * p.g_inv) >> 10) : m & (PP - 1); };
   // The operands that do not change are fetched ahead: what follows waits for the page counts first (a load of memory that the SM has not
   // touched takes 1 - 2 us).  One line per thread.  (A block under a sliding window is short: 2 x 2048 rows 343 -> 338 us.  Long ones gain nothing.)
   if constexpr (MODE == MODE_SLIDING) {
@@ -142,37 +147,35 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     else if (tid >= 128 && tid < 132) at = reinterpret_cast<const uint8_t*>(p.signs) + (tid - 128) * 128;
     else if (tid >= 256 && tid < 512) {
       const int m = (tid - 256) >> 1;
-      at = reinterpret_cast<const uint8_t*>(p.q + (((int64_t)b * H + h * G + m / PP) * p.n_q + min(i0 + m % PP, p.n_q - 1)) * HEAD_DIM) + ((tid & 1) << 7);
+      at = reinterpret_cast<const uint8_t*>(p.q + (((int64_t)b * H + h * G + head_of(m)) * p.n_q + min(i0 + pos_of(m), p.n_q - 1)) * HEAD_DIM) + ((tid & 1) << 7);
     }
     if (at) asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
   }
-  // MODE_PREFIX: row m is query head m % G of the group's member i0 + m / G (any G up to 8; 128 - PP * G rows idle)
   const int4 group = MODE == MODE_PREFIX ? reinterpret_cast<const int4*>(p.groups)[b] : make_int4(0, 0, b, 0);
   const int m0 = group.x, n_members = group.y - group.x, first_member = group.z;
   if (MODE == MODE_PREFIX) asm volatile("griddepcontrol.launch_dependents;");  // the kernel that streams the pages behind the prefixes
   if (MODE == MODE_PREFIX && i0 >= n_members) return;
 
-  const int64_t pq_min = p.q_pos0 + i0;                                // first query position of the CTA
-  const int64_t pq_max = p.q_pos0 + min(i0 + PP, p.n_q) - 1;           // last one
+  // Positions relative to pos_offset, the first committed token's (32 bits: a context is shorter than 2^30 tokens)
+  const int x_min = p.q_rel + i0, x_max = p.q_rel + min(i0 + PP, p.n_q) - 1;  // first and last query position of the CTA
   const int n_pg = MODE == MODE_PREFIX ? min(max(group.w, 0), p.n_pages[first_member]) : p.n_pages[b];
-  const int64_t vis = MODE == MODE_PREFIX ? (int64_t)n_pg * 128 : pq_max - p.pos_offset;
-  if (MODE != MODE_CAUSAL && FRAG && tid == 0 && min((int64_t)n_pg, vis / 128 + 1) > p.rope_pages && atomicCAS(p.status, 0, 3) == 0)
-    p.status[1] = p.rope_pages, p.status[2] = n_pg;
-  const int n_last = (vis < 0) ? 0 : (int)min((int64_t)(FRAG ? min(n_pg, p.rope_pages) : n_pg), vis / 128 + 1);  // pages whose first token the last position sees
+  const int visible = MODE == MODE_PREFIX ? n_pg : x_max < 0 ? 0 : min(n_pg, (x_max >> 7) + 1);  // pages whose first token the last position sees
+  if (MODE != MODE_CAUSAL && FRAG && tid == 0 && visible > p.rope_pages && atomicCAS(p.status, 0, 3) == 0)
+    p.status[1] = p.rope_pages, p.status[2] = visible;
+  const int n_last = FRAG ? min(visible, p.rope_pages) : visible;
   // MODE_SLIDING: of those, the sinks' pages [0, keep) and the pages from the first row's window on; the gap between them is left out
-  const int64_t lo_min = MODE == MODE_SLIDING ? max((int64_t)0, pq_min - p.window + 1) : 0, lo_max = MODE == MODE_SLIDING ? pq_max - p.window + 1 : 0;
-  const int keep = MODE == MODE_SLIDING ? (int)min((int64_t)n_last, (p.sinks + 127) / 128) : 0;
-  const int gap = MODE == MODE_SLIDING ? max(0, (int)min((int64_t)n_last, lo_min / 128) - keep) : 0;
+  const int lo_min = MODE == MODE_SLIDING ? max(0, x_min - p.window + 1) : 0, lo_max = MODE == MODE_SLIDING ? x_max - p.window + 1 : 0;
+  const int keep = MODE == MODE_SLIDING ? min(n_last, (p.sinks + 127) >> 7) : 0;
+  const int gap = MODE == MODE_SLIDING ? max(0, min(n_last, lo_min >> 7) - keep) : 0;
   const int NPv = n_last - gap;
   // this CTA's share of them: pages T0 .. T0 + NP - 1; the window goes with the last share
-  const int per_share = (NPv + n_split - 1) / n_split;
+  const int per_share = n_split == 1 ? NPv : (NPv + n_split - 1) / n_split;
   const int T0 = min(NPv, share * per_share), NP = min(NPv, T0 + per_share) - T0;
   auto page_of = [&](int n) { return MODE == MODE_SLIDING && T0 + n >= keep ? T0 + n + gap : T0 + n; };  // page of this share's tile n
   const int tl = MODE == MODE_PREFIX ? 0 : p.tail_len ? min(p.tail_len[b], p.tail_cap) : 0;
-  const int64_t tail_pos0 = p.pos_offset + (int64_t)n_pg * 128;
-  const int NW = (share == n_split - 1 && tl > 0 && pq_max >= tail_pos0) ? (int)((min((int64_t)tl, pq_max - tail_pos0 + 1) + 127) / 128) : 0;
+  const int tail_x0 = n_pg * 128;
+  const int NW = (share == n_split - 1 && tl > 0 && x_max >= tail_x0) ? (min(tl, x_max - tail_x0 + 1) + 127) >> 7 : 0;
   const int NT = NP + NW;
-  const int64_t page_pos0 = p.pos_offset + (int64_t)T0 * 128;  // position of the first key of this share (MODE_SLIDING: see page_of)
 
   const int32_t* table = p.page_table + (int64_t)first_member * p.table_stride;
   auto copy_tile = [&](int stage, int slot) {  // one thread: a page's coefficients and its block of this head
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     __syncwarp();
   } else {
     // every load of a thread is in flight before its first store
-    constexpr int ST = P5_THREADS - 32, NQ = (128 * 18 + ST - 1) / ST;
+    constexpr int ST = P5_THREADS - 32, NQ = (128 * 16 + ST - 1) / ST;
     const int st = tid - (warp > 16 ? 32 : 0);
     if (warp == 17) {
       tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
@@ -216,27 +219,28 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     }
     uint4 qv[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {  // row m = (query head m / PP, position i0 + m % PP)
-      const int o = st + i * ST, m = o / 18, c8 = o % 18;
-      qv[i] = make_uint4(c8 == 16 ? 0x3C003C00u : 0u, 0u, 0u, 0u);  // K index 128, 129: ones against the norm pair
-      if (c8 < 16 && m < 128) {
-        const int qi = MODE == MODE_PREFIX ? m % G : m / PP, ip = MODE == MODE_PREFIX ? min(i0 + m / G, n_members - 1) : min(i0 + m % PP, p.n_q - 1);
-        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)__ldg(p.members + m0 + ip) * H + h * G + qi : ((int64_t)b * H + h * G + qi) * p.n_q + ip;
+    for (int i = 0; i < NQ; ++i) {  // 16 bytes c8 of row m
+      const int o = st + i * ST, m = o >> 4, c8 = o & 15;
+      if (m < 128) {
+        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)__ldg(p.members + m0 + min(i0 + pos_of(m), n_members - 1)) * H + h * G + head_of(m)
+                                                 : ((int64_t)b * H + h * G + head_of(m)) * p.n_q + min(i0 + pos_of(m), p.n_q - 1);
         qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM) + c8);
       }
     }
     const uint4 bv = st < 128 * (RANK / 8) ? __ldg(reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK) + st) : make_uint4(0u, 0u, 0u, 0u);
     static_assert(128 * (32 / 8) <= ST, "one piece of the basis per thread");
     const float sv = st < 128 ? __ldg(p.signs + st) : 0.f;
+    if (st < 128) {  // K index 128, 129 of Q: ones against the norm pair; 130 .. 143 of Q and 136 .. 143 of both key buffers: zero for good
+      const int at = (st >> 3) * OP_SBO + (st & 7) * 16;
+      *reinterpret_cast<uint4*>(qop + at + 16 * 128) = make_uint4(0x3C003C00u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(qop + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(kop0 + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
+      *reinterpret_cast<uint4*>(kop0 + OP_BYTES + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int o = st + i * ST, m = o / 18, c8 = o % 18;
-      if (m >= 128) break;
-      *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = qv[i];
-      if (c8 == 17) {  // K index 136 .. 143 of both key buffers: zero for good
-        *reinterpret_cast<uint4*>(kop0 + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(kop0 + OP_BYTES + (m >> 3) * OP_SBO + 17 * 128 + (m & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
+      const int o = st + i * ST, m = o >> 4, c8 = o & 15;
+      if (m < 128) *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = qv[i];
     }
     if (st < 128 * (RANK / 8)) {
       const int c = st / (RANK / 8), i8 = st % (RANK / 8);
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P5_REG_KEY));
     const int wq = warp & 3, k0 = 2 * (warp >> 2), row = 32 * wq + lane;
     const uint32_t tk = tmem + TM_KL + ((uint32_t)(32 * wq) << 16);
-    const int grp = row / g.group;
+    const int grp = row >> (31 - __clz(g.group));
     const __half2 c1032 = __floats2half2_rn(1032.f, 1032.f);
     const __half2 c16th = __floats2half2_rn(0.0625f, 0.0625f);
     const __half2 cm72 = __floats2half2_rn(-72.f, -72.f);
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         const uint4* ps = pc + ROPE_FRAG_UINT4 / 2;
         cs4[kk][0] = pc[0], cs4[kk][1] = pc[32], sn4[kk][0] = ps[0], sn4[kk][1] = ps[32];
       } else {
-        const int64_t pos = MODE == MODE_SLIDING ? p.pos_offset + (int64_t)page_of(n) * 128 + row : page_pos0 + (int64_t)n * 128 + row;
+        const int64_t pos = p.pos_offset + page_of(n) * 128 + row;
         const uint4* pc = reinterpret_cast<const uint4*>(p.rope_cos + pos * HEAD_DIM + 16 * (k0 + kk));
         const uint4* ps = reinterpret_cast<const uint4*>(p.rope_sin + pos * HEAD_DIM + 16 * (k0 + kk));
         cs4[kk][0] = pc[0], cs4[kk][1] = pc[1], sn4[kk][0] = ps[0], sn4[kk][1] = ps[1];
@@ -369,7 +373,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       } else {
         // window tile: the keys are stored rotated; rows past the window's length are zero; norm 1
         const int t0 = (n - NP) * 128;
-        const bool valid = t0 + row < tl && (MODE != MODE_SLIDING || tail_pos0 + t0 + row >= lo_min || tail_pos0 + t0 + row < p.sinks);
+        const bool valid = t0 + row < tl && (MODE != MODE_SLIDING || tail_x0 + t0 + row >= lo_min || tail_x0 + t0 + row < p.sinks);
         const uint4* src = reinterpret_cast<const uint4*>(kt + (int64_t)(t0 + row) * HEAD_DIM);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -446,7 +450,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = t0 + 8 * (i0_ + i) + tr;
-            const bool in = t < tl && (MODE != MODE_SLIDING || tail_pos0 + t >= lo_min || tail_pos0 + t < p.sinks);
+            const bool in = t < tl && (MODE != MODE_SLIDING || tail_x0 + t >= lo_min || tail_x0 + t < p.sinks);
             rows[i] = in ? reinterpret_cast<const uint4*>(vt + (int64_t)t * HEAD_DIM)[c8] : make_uint4(0u, 0u, 0u, 0u);
           }
 #pragma unroll
@@ -474,13 +478,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P5_REG_SOFTMAX));
     const int wq = warp & 3, row = 32 * wq + lane, hf = (warp - 8) >> 2;
     const uint32_t tl_ = tmem + ((uint32_t)(32 * wq) << 16);
-    const int qi = MODE == MODE_PREFIX ? row % G : row / PP, ip = MODE == MODE_PREFIX ? i0 + row / G : i0 + row % PP;
-    // positions relative to page_pos0: of this row and the CTA's first row, plus one; of the first key in this row's window and in the last row's
-    const int64_t pq = p.q_pos0 + ip;
-    auto rel32 = [](int64_t x) { return (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, x)); };
-    const int row_rel = rel32(pq - page_pos0 + 1), first_rel = rel32(pq_min - page_pos0 + 1);
-    const int win_row = MODE == MODE_SLIDING ? rel32(pq - p.window + 1 - page_pos0) : 0, win_max = MODE == MODE_SLIDING ? rel32(lo_max - page_pos0) : 0;
-    const int sinks_rel = MODE == MODE_SLIDING ? rel32(p.sinks - page_pos0) : 0;
+    const int qi = head_of(row), ip = i0 + pos_of(row);
+    const int x = p.q_rel + ip, win = MODE == MODE_SLIDING ? x - p.window + 1 : 0;  // this row's position, the first of its window
     const bool in_group = MODE == MODE_PREFIX && row < PP * G && ip < n_members;
     const int my_seq = in_group ? p.members[m0 + ip] : 0;  // for the record at the end
     float m = -1e30f;
@@ -559,14 +558,13 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     PROF_DECL(8)
     for (int n = 0; n < NT && alive; ++n) {  // half tile u = (tile n, half hf): tokens 64 hf .. 64 hf + 63
       const int u = 2 * n + hf, e = n & 1;
-      // Everything relative to the first key of the half (32 bits: a context is shorter than 2^31 tokens).  Keys [0, jl) of the half are at positions
-      // up to this row's; MODE_SLIDING: of those it sees [0, js) as sinks and [jw, jl) as its window.
-      const int from = (n < NP ? (MODE == MODE_SLIDING ? page_of(n) - T0 : n) : n_pg - T0 + (n - NP)) * 128 + 64 * hf;  // behind page_pos0
+      // the half's first key; of its keys, [0, jl) are at positions up to this row's, and under a sliding window [0, js) are sinks, [jw, jl) the window
+      const int from = (n < NP ? page_of(n) : n_pg + n - NP) * 128 + 64 * hf;
       const int n_valid = (n < NP) ? 64 : max(0, min(64, tl - (n - NP) * 128 - 64 * hf));
-      const bool masked = MODE != MODE_PREFIX && (first_rel - from < 64 || n_valid < 64 ||
-                                                  (MODE == MODE_SLIDING && from < win_max && from + 64 > sinks_rel));  // the same for the whole CTA
-      const int jl = max(0, min(n_valid, row_rel - from));
-      const int js = MODE == MODE_SLIDING ? sinks_rel - from : 0, jw = MODE == MODE_SLIDING ? win_row - from : 0;
+      const bool masked = MODE != MODE_PREFIX && (x_min + 1 - from < 64 || n_valid < 64 ||
+                                                  (MODE == MODE_SLIDING && from < lo_max && from + 64 > p.sinks));  // the same for the whole CTA
+      const int jl = max(0, min(n_valid, x + 1 - from));
+      const int js = MODE == MODE_SLIDING ? p.sinks - from : 0, jw = MODE == MODE_SLIDING ? win - from : 0;
       const uint32_t tS = tl_ + TM_S + 64 * hf, tP = tl_ + TM_P + 32 * hf;
       if (n == NP && NP > 0) {  // first window tile after pages: leave the rotated space of the value codec
         if (!(warp_wait(&sh->odone[0], (uint32_t)(n - 1) & 1u, p.status, 46) && warp_wait(&sh->odone[1], (uint32_t)(n - 1) & 1u, p.status, 46))) {
@@ -827,7 +825,13 @@ static size_t p5_smem_bytes(int rank, int group) {
 }
 
 template <int RANK, bool FRAG, int MODE>
-static int launch_p5(const PrefillParams& prm, dim3 grid, size_t smem, cudaStream_t s) {
+static int launch_p5(const PrefillParams& given, dim3 grid, size_t smem, cudaStream_t s) {
+  PrefillParams prm = given;
+  // rows further than 2^30 from the first key see as much as at that distance: what is held is shorter by far
+  const int64_t rel = prm.q_pos0 - prm.pos_offset, most = 1 << 30;
+  prm.q_rel = (int)(rel < -most ? -most : rel > most - prm.n_q ? most - prm.n_q : rel);
+  prm.pp = 128 / prm.g.n_q_groups, prm.pp_log = 0, prm.g_inv = (1024 + prm.g.n_q_groups - 1) / prm.g.n_q_groups;
+  while ((2 << prm.pp_log) <= prm.pp) ++prm.pp_log;
   static PerDeviceOnce configured;
   if (configured.first()) {
     cudaError_t e = cudaFuncSetAttribute((k2b_prefill_t5_kernel<RANK, FRAG, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);

@@ -39,11 +39,14 @@ struct PrefillParams {
   int rope_pages;
   // MODE_SLIDING: a row at position x sees the keys of (x - window, x] and those below `sinks`; pages that no row of a block sees are
   // not touched
-  int64_t window, sinks;
+  int window, sinks;
   // MODE_PREFIX: single-token queries q (batch, heads, 128) of the sequences members[begin .. end - 1] over the first `pages` pages of
   // the page-table row of `first` (one of them), which all share; groups[z] = {begin, end, first, pages}, 16-byte aligned
   const int32_t* members;
   const int32_t* groups;
+  // tcgen05 kernel, set by its launchers: first query position relative to pos_offset; query positions (sequences) per CTA, 128 / n_q_groups, and
+  // its logarithm where it is a power of two; 1024 / n_q_groups rounded up (m * g_inv >> 10 = m / n_q_groups for m < 128)
+  int q_rel, pp, pp_log, g_inv;
 };
 constexpr int MODE_CAUSAL = 0, MODE_PREFIX = 1, MODE_SLIDING = 2;
 constexpr int ROPE_FRAG_UINT4 = 2048;  // per page: [cos, sin][chunk of 16 pairs][32 tokens x 4][half of the chunk][lane]
