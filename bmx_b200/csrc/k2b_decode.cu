@@ -1015,6 +1015,14 @@ static int check_step(const bmxk_k2b_geom* g, const void* q, const void* pages, 
   return BMXK_OK;
 }
 
+// What the steps under a sliding window and behind shared prefixes read and write 16 bytes at a time.
+static int check_aligned(const char* who, const void* q, const void* basis_f16, const void* k_tail, const void* v_tail, const void* workspace,
+                         const void* out) {
+  BMXK_REQUIRE((((uintptr_t)q | (uintptr_t)basis_f16 | (uintptr_t)k_tail | (uintptr_t)v_tail | (uintptr_t)workspace | (uintptr_t)out) & 15) == 0,
+               "%s: q, basis, windows, workspace and out must be 16-byte aligned", who);
+  return BMXK_OK;
+}
+
 // One decode step over the pages that `walk` names (at most walk_pages of a sequence), the window and, for WALK_OWN, the records of the
 // shared prefixes; the entry points below check what is theirs.
 static int decode_step(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
@@ -1101,6 +1109,10 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
   BMXK_REQUIRE(g != nullptr && g->layout == 1 && g->page == 128, "bmxk_k2b_decode_sliding: pools of layout 1 (128-token pages in row order) only");
   BMXK_REQUIRE(window >= 1 && sinks >= 0, "bmxk_k2b_decode_sliding: window=%lld sinks=%lld (a query sees itself: window >= 1)", (long long)window,
                (long long)sinks);
+  const int bad = check_aligned("bmxk_k2b_decode_sliding", q, basis_f16, k_tail, v_tail, workspace, out);
+  if (bad) return bad;
+  if (window > (1LL << 40)) window = 1LL << 40;  // longer than any context: no sum below overflows
+  if (sinks > (1LL << 40)) sinks = 1LL << 40;
   K2bWalk w = {};
   w.tail_len = tail_cap > 0 ? tail_len : nullptr, w.tail_cap = tail_cap, w.window = window, w.sinks = sinks;
   const int64_t most = (sinks + 127) / 128 + (window - 1) / 128 + 2;  // pages that hold a visible token
@@ -1138,6 +1150,8 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   const int bad = check_step(g, q, pages, coefs, basis_f16, page_table, n_pages, batch, max_pages, rope_cos, rope_sin, k_tail, v_tail, tail_len,
                              tail_cap, v_lut, signs, workspace, workspace_bytes, out, out_dtype, nullptr, 3);
   if (bad) return bad;
+  const int off = check_aligned("bmxk_k2b_decode_shared", q, basis_f16, k_tail, v_tail, workspace, out);
+  if (off) return off;
   const bool prefixes = n_groups > 0 && max_members > 0 && max_pages > 0;
   float* part = reinterpret_cast<float*>((uint8_t*)workspace + (bmxk_k2b_decode_workspace_bytes(g, batch, 0) + 255) / 256 * 256);
   if (prefixes) {

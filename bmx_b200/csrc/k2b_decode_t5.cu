@@ -153,6 +153,10 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   // load of memory that the SM has not touched takes 1 - 3 us, and the first tile is most of such a walk).
   int slot = 0;
   uint32_t csw = 0, snw = 0, x1[GQ], x2[GQ];
+  const bool q_words = WALK != WALK_ALL || (reinterpret_cast<uintptr_t>(p.q) & 3) == 0;  // the plain step takes queries that begin on any fp16
+  auto query_word = [&](const __half* at) {
+    return q_words ? *reinterpret_cast<const uint32_t*>(at) : h2_as_u32(__halves2half2(at[0], at[1]));
+  };
   auto load_tile = [&](const TileCursor& cur) {
     const int b = cur.b, h = cur.h, j = page_of(b, cur.j);
     const int64_t t0 = p.pos_offset + (int64_t)j * TILE_TOKENS;
@@ -165,9 +169,8 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
     snw = reinterpret_cast<const uint32_t*>(p.rope_sin + t0 * HEAD_DIM)[lane];
 #pragma unroll
     for (int qi = 0; qi < GQ; ++qi) {
-      const uint32_t* qw = reinterpret_cast<const uint32_t*>(qsrc + qi * HEAD_DIM);
-      x1[qi] = (qi < G) ? qw[lane] : 0u;
-      x2[qi] = (qi < G) ? qw[lane + 32] : 0u;
+      x1[qi] = (qi < G) ? query_word(qsrc + qi * HEAD_DIM + 2 * lane) : 0u;
+      x2[qi] = (qi < G) ? query_word(qsrc + qi * HEAD_DIM + 2 * lane + 64) : 0u;
     }
   };
   if (WALK != WALK_ALL && warp >= 26) {

@@ -85,9 +85,9 @@ extern "C" int bmxk_copy_slots(int n_arrays, const void* const* src, void* const
                  (long long)dst_stride[a]);
     BMXK_REQUIRE((((uintptr_t)src[a] | (uintptr_t)dst[a] | (uintptr_t)bytes[a] | (uintptr_t)src_stride[a] | (uintptr_t)dst_stride[a]) & 15) == 0,
                  "bmxk_copy_slots: array %d: pointers, strides and sizes must be multiples of 16 bytes", a);
+    BMXK_REQUIRE(src_stride[a] <= (1LL << 32) && dst_stride[a] <= (1LL << 32), "bmxk_copy_slots: array %d: slots more than 4 GiB apart", a);
     arr[a] = CopyArray{(const uint8_t*)src[a], (uint8_t*)dst[a], src_stride[a], dst_stride[a], bytes[a], (int)chunks};
     chunks += (bytes[a] + COPY_CHUNK - 1) / COPY_CHUNK;
-    BMXK_REQUIRE(chunks <= (1 << 20), "bmxk_copy_slots: slots of more than 16 GiB");
   }
   // Arrays may coincide (a copy inside one pool) but not overlap in any other way: what one pair writes another one could read.
   auto overlap = [](const uint8_t* p, int64_t pn, const uint8_t* q, int64_t qn) { return p < q + qn && q < p + pn; };

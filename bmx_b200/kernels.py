@@ -353,14 +353,15 @@ def rope_fragments(rope_cos: torch.Tensor, rope_sin: torch.Tensor, n_pages: int)
 
 
 @functools.lru_cache(maxsize=None)
-def _sm_count(device: torch.device) -> int:
+def sm_count(device: torch.device) -> int:
+    """Multiprocessors of a device."""
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
 def split_walk(ctas: int, pages: int, device, most: int = 64) -> int:
     """Shares of a page walk of `pages` pages that `ctas` CTAs would each make whole: the number that makes (waves of CTAs) x (pages
     per share + the CTA's set-up, about four pages' worth) smallest."""
-    n_sm = _sm_count(torch.device(device))
+    n_sm = sm_count(torch.device(device))
     best, best_cost = 1, None
     for s in range(1, max(1, min(most, pages)) + 1):
         cost = -(-ctas * s // n_sm) * (-(-pages // s) + 4)
@@ -371,7 +372,7 @@ def split_walk(ctas: int, pages: int, device, most: int = 64) -> int:
 
 def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int, basis_f16: torch.Tensor | None,
                 rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, k_tail: torch.Tensor | None, v_tail: torch.Tensor | None,
-                tail_len: torch.Tensor | None, signs: torch.Tensor) -> int:
+                tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor) -> int:
     """What every step over a k2b pool asks of its tensors; returns the window's capacity."""
     g = pool.geom
     h_kv, batch, half, i32 = g.h_kv, q.shape[0], torch.float16, torch.int32
@@ -381,6 +382,7 @@ def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_page
     assert n_pages.dtype is i32 and n_pages.shape == (batch,) and n_pages.is_contiguous()
     assert 0 <= max_pages <= columns, f"max_pages={max_pages}: the page table has {columns} columns"
     assert signs.dtype is torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
+    assert v_lut.dtype is i32 and v_lut.numel() == 4 and not v_lut.is_cuda, "v_lut: v_lut_tensor(), on the host"
     if max_pages > 0:
         assert basis_f16.dtype is half and basis_f16.is_contiguous() and basis_f16.numel() == h_kv * HEAD_DIM * g.rank
         for t in (rope_cos, rope_sin):
@@ -413,7 +415,7 @@ def k2b_decode_sliding(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, 
     g = pool.geom
     assert q.dim() == 3
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs, workspace):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_sliding", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
              page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(rope_cos), _addr(rope_sin), _addr(k_tail), _addr(v_tail), _addr(tail_len),
@@ -434,7 +436,7 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
     assert q.dim() == 4 and q.shape[2] >= 1
     batch, n_q = q.shape[0], q.shape[2]
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, status):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert status.numel() * status.element_size() >= 16 and status.is_contiguous()
         rope_pages = _check_fragments(rope, 0)
         out = _check_out(out, q, (torch.float16,))
@@ -504,7 +506,7 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
     assert q.dim() == 3 and groups.batch == q.shape[0], f"groups of a batch of {groups.batch}, queries of {q.shape[0]}"
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, workspace,
                        groups.skip):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs)
+        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
         rope_pages = _check_fragments(rope, groups.max_prefix)
         out = _check_out(out, q, (torch.float16, torch.float32))

@@ -30,6 +30,7 @@ class PageAllocator:
         self._owned: dict[object, list[int]] = {}
         self._refs: dict[int, int] = {}                # slot -> sequences that hold it
         self.peak_in_use = 0
+        self.version = 0                               # changes with every change of who holds what
 
     def alloc(self, seq, n: int, places: list[int] | None = None, pages: int | None = None) -> list[int]:
         """n more slots for sequence `seq`; raises MemoryError (and changes nothing) if the pool cannot hold them.  With places, the
@@ -37,6 +38,7 @@ class PageAllocator:
         if n > len(self._free):
             raise MemoryError(f"page pool exhausted: {n} slots wanted, {len(self._free)} of {self.n_slots} free")
         got = [self._free.pop() for _ in range(n)]
+        self.version += bool(got or pages)
         for s in got:
             self._refs[s] = 1
         held = got
@@ -51,6 +53,7 @@ class PageAllocator:
     def _give_back(self, slots: list[int]) -> int:
         """One holder less for each slot, in order; returns how many are free again."""
         n = 0
+        self.version += bool(slots)
         for s in slots:
             self._refs[s] -= 1
             if self._refs[s] == 0:
@@ -68,6 +71,7 @@ class PageAllocator:
         if self._owned.get(other):
             raise ValueError(f"sequence {other!r} holds slots already")
         slots = self._owned.get(seq, [])
+        self.version += 1
         for s in slots:
             if s >= 0:
                 self._refs[s] += 1
@@ -92,6 +96,7 @@ class PageAllocator:
         """Renumbers the held slots to 0 .. in_use - 1 and returns the (from, to) lists of those that have to be copied: the ones
         beyond, into the holes below, so that no slot is both read and written."""
         m = self.in_use
+        self.version += 1
         holes = sorted(s for s in self._free if s < m)
         moved = sorted(s for s in self._refs if s >= m)
         new = dict(zip(moved, holes))
@@ -145,9 +150,11 @@ class PagedK2bLayer:
     that fall between the two are freed as sequences grow.  `compact` and `resize` close the holes that finished sequences leave.
     """
 
-    # Pages of a shared prefix from which attending it once for `n` sequences beats streaming it n times (see _prefix_groups).
-    SHARED_MIN_ROWS = 12
-    SHARED_MIN_PAGES = 8
+    # 128-token tiles per SM that attending shared prefixes once has to save over streaming them for every sequence.  Its launch and the set-up of
+    # its blocks cost about 5 us.  Measured at 8 KV heads x 4 query heads, shared against streamed: 4 sequences x 32 pages (5.2 tiles per SM
+    # saved) 21 against 22 us, 8 x 8 pages (3.0) 19 against 18, 3 x 32 (3.5) 21 against 20, 8 x 32 (12) 21 against 28, 32 x 256 46 against 398;
+    # at 1 and 8 query heads per KV head the two meet at 4 - 5 and 3.
+    SHARED_MIN_TILES = 5
 
     def __init__(self, geom, n_slots: int, max_seqs: int, recent_window: int, device, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
                  *, v_seed: int = 0, max_pages_per_seq: int = 1024, sliding_window: int | None = None, sinks: int = 0):
@@ -177,7 +184,7 @@ class PagedK2bLayer:
         self._committed: dict[object, int] = {}
         self._tail: dict[object, int] = {}
         self._ws: dict[int, torch.Tensor] = {}      # decode workspaces by batch size
-        self._groups: tuple | None = None           # the last step's page tables, its prefix groups and their workspace
+        self._plan: tuple | None = None             # (what it holds for, page table, page counts, window rows, prefix groups, workspace) of a step
         self._rope_frag: torch.Tensor | None = None  # rotation tables in the prefill kernel's order, as far as prefixes reach
 
     # ---- bookkeeping ------------------------------------------------------------------------
@@ -267,7 +274,8 @@ class PagedK2bLayer:
             assert len(old) + n_flush <= self.max_pages, "sequence longer than max_pages_per_seq pages"
             if self.basis_f32 is None:
                 self.set_basis(fit_basis(self.geom, src_k[:, : self.page]))
-        self.alloc.release(seq, *gone)
+        if gone[0] < gone[1]:
+            self.alloc.release(seq, *gone)
         if n_flush > 0:
             got = dict(zip(kept, self.alloc.alloc(seq, len(kept), [p - p0 for p in kept], n_flush)))
             k_all, v_all = src_k[None], val[None].to(src_k.dtype)
@@ -285,57 +293,57 @@ class PagedK2bLayer:
 
     # ---- decode -----------------------------------------------------------------------------
     def _prefix_groups(self, slots: list) -> tuple[list, list]:
-        """(members, prefix pages) of the sequences that begin with the same slots.  A group is worth a pass of its own when it has
-        enough query rows per KV head (the prefix kernel's cost does not depend on them, the streaming kernel's grows with every
-        sequence) and enough pages."""
+        """(members, prefix pages) of the sequences that begin with the same slots, where attending their prefixes once pays."""
         first: dict[int, list[int]] = {}
         for i, s in enumerate(slots):
             if s:
                 first.setdefault(s[0], []).append(i)
         members, pages = [], []
         for rows in first.values():
-            if len(rows) * self.geom.n_q_groups < self.SHARED_MIN_ROWS or len(rows) < 2:
+            if len(rows) < 2:
                 continue
             a, n = slots[rows[0]], min(len(slots[r]) for r in rows)
             for r in rows[1:]:
                 s = slots[r]
                 if s[:n] != a[:n]:
                     n = next(j for j in range(n) if s[j] != a[j])
-            if n >= self.SHARED_MIN_PAGES:
-                members.append(rows)
-                pages.append(n)
-        return members, pages
+            members.append(rows)
+            pages.append(n)
+        saved = sum((len(m) - 1) * n for m, n in zip(members, pages)) * self.geom.h_kv
+        return (members, pages) if saved >= self.SHARED_MIN_TILES * K.sm_count(self.device) else ([], [])
 
     def decode(self, seqs: list, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """q (len(seqs), heads, 128) fp16: one fused decode step over those sequences, each with its own pages and window; a prefix
         that several of them share is read once."""
         n = len(seqs)
-        rows = torch.tensor([self._rows[s] for s in seqs], device=self.device)
-        slots = [self.alloc.slots(s) for s in seqs]
-        counts = [len(s) for s in slots]
-        max_pg = max(1, max(counts))
-        table = torch.tensor([s + [0] * (max_pg - len(s)) for s in slots], dtype=torch.int32).to(self.device)
-        both = torch.tensor(counts + [self._tail[s] for s in seqs], dtype=torch.int32).to(self.device)
-        n_pages, tail = both[:n], both[n:]
-        max_walk = max_pg if any(counts) else 0
+        holds = (tuple(self._rows[s] for s in seqs), tuple(seqs), self.alloc.version, self.SHARED_MIN_TILES)
+        if self._plan is None or self._plan[0] != holds:
+            slots = [self.alloc.slots(s) for s in seqs]
+            counts = [len(s) for s in slots]
+            max_pg = max(1, max(counts))
+            table = torch.tensor([s + [0] * (max_pg - len(s)) for s in slots], dtype=torch.int32).to(self.device)
+            ints = torch.tensor(counts, dtype=torch.int32).to(self.device)
+            groups = ws = None
+            if self.sliding_window is None and self.geom.layout == 1:
+                members, pages = self._prefix_groups(slots)
+                if members:
+                    groups = K.PrefixGroups(self.geom, n, members, pages, self.device)
+                    ws = K.decode_shared_workspace(self.geom, n, groups, self.device)
+                    if self._rope_frag is None or self._rope_frag.shape[0] < groups.max_prefix:
+                        most = self.rope_cos.shape[0] // 128
+                        self._rope_frag = K.rope_fragments(self.rope_cos, self.rope_sin, min(most, 2 * groups.max_prefix))
+            self._plan = (holds, table, ints, torch.tensor(holds[0], device=self.device), groups, ws, max_pg if any(counts) else 0)
+        _, table, n_pages, rows, groups, ws, max_walk = self._plan
+        tail = torch.tensor([self._tail[s] for s in seqs], dtype=torch.int32).to(self.device)
         basis16 = self.basis_f16 if self.basis_f16 is not None else torch.zeros(self.geom.h_kv * HEAD_DIM, self.geom.rank, dtype=torch.float16,
                                                                                  device=self.device)
         tails = (self.k_win[rows].contiguous(), self.v_win[rows].contiguous(), tail)
         last = (self.v_lut, self.signs, self.sm_scale)
-        if self.sliding_window is None and self.geom.layout == 1:
-            if self._groups is None or self._groups[0] != slots:
-                members, pages = self._prefix_groups(slots)
-                groups = K.PrefixGroups(self.geom, n, members, pages, self.device) if members else None
-                self._groups = (slots, groups, K.decode_shared_workspace(self.geom, n, groups, self.device) if groups else None)
-            _, groups, ws = self._groups
-            if groups is not None:
-                if self._rope_frag is None or self._rope_frag.shape[0] < groups.max_prefix:
-                    most = self.rope_cos.shape[0] // 128
-                    self._rope_frag = K.rope_fragments(self.rope_cos, self.rope_sin, min(most, 2 * groups.max_prefix))
-                return K.k2b_decode_shared(self.pool, q, basis16, table, n_pages, max_walk, groups, self.rope_cos, self.rope_sin, self._rope_frag,
-                                           *tails, *last, ws, out=out)
+        if groups is not None:
+            return K.k2b_decode_shared(self.pool, q, basis16, table, n_pages, max_walk, groups, self.rope_cos, self.rope_sin, self._rope_frag, *tails, *last,
+                                       ws, out=out)
         if n not in self._ws:
-            self._ws[n] = K.decode_workspace(self.geom, n, max_pg, self.device)
+            self._ws[n] = K.decode_workspace(self.geom, n, table.shape[1], self.device)
         if self.sliding_window is not None:
             return K.k2b_decode_sliding(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, self._ws[n],
                                         self.sliding_window, self.sinks, out=out)

@@ -150,6 +150,8 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
  * total - 1, total = 128 * n_pages[s] + tail_len[s]) sees those at positions >= total - window (window >= 1: itself among them) and those
  * < sinks.  Arguments as in bmxk_k2b_decode (no pos_offset, no partial states); layout 1 only.  Pages without a visible token are not
  * read and their page-table entries may be anything: a caller frees them.  No per-step argument.  A sequence that holds nothing gives 0.
+ * q, basis, windows, workspace (bmxk_k2b_decode_workspace_bytes) and out are 16-byte aligned; calls that may run at the same time need
+ * workspaces of their own.
  * (bmx's cache attends to everything it holds: src/bmx/cache/chunked_attention.py:398-530; a model's sliding layers have no path there.) */
 int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
                             const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const void* rope_cos,
@@ -164,7 +166,7 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
  * arguments and result these are (no pos_offset, no partial states).  skip, members, groups: int32 device arrays; max_members: the
  * largest group.  rope_frag: bmxk_k2b_rope_fragments of rope_pages pages (every prefix has to lie within, see the status word (3,
  * rope_pages, pages)), or null: the tables are read as they are, about a quarter slower.  Layout 1, sm_scale > 0.  workspace:
- * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once.  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every
+ * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once; alignment and concurrency as above.  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every
  * sequence has a cache of its own.) */
 size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split);
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,

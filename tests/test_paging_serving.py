@@ -151,6 +151,7 @@ class Bench:
 @pytest.mark.gpu
 def test_forks_share_their_prompt_and_go_their_own_ways():
     b = Bench(slots=40)
+    b.layer.SHARED_MIN_TILES = 0                          # share whatever can be shared
     b.start("doc", 0, 1500, 700)                          # 11 pages and 92 tokens in the window
     assert b.layer.alloc.in_use == 11
     kids = [f"k{i}" for i in range(9)]
@@ -162,9 +163,17 @@ def test_forks_share_their_prompt_and_go_their_own_ways():
     b.start("other", 3, 300)
     order = kids[:4] + ["other", "doc"] + kids[4:]
     b.check(order)
-    assert b.layer._groups[1] is not None and b.layer._groups[1].max_members == 10     # the prompt was attended once
-    b.check(["k1", "k1", "k8"])                           # the same sequence twice; too few rows to share
-    assert b.layer._groups[1] is None or b.layer._groups[1].n_groups <= 1
+    assert b.layer._plan[4] is not None and b.layer._plan[4].max_members == 10     # the prompt was attended once
+    plan = b.layer._plan
+    b.feed("k1", 2, 1)                                    # a token that commits no page: tables and groups stay
+    b.check(order)
+    assert b.layer._plan is plan
+    b.check(["k1", "k1", "k8"])                           # the same sequence twice
+    assert b.layer._plan[4].max_members == 3
+    b.layer.SHARED_MIN_TILES = 5                          # too little to save here
+    b.check(["doc"] + kids)
+    assert b.layer._plan[4] is None
+    b.layer.SHARED_MIN_TILES = 0
     before = b.layer.alloc.in_use
     freed = b.layer.drop_sequence("doc")
     assert freed == 0 and b.layer.alloc.in_use == before  # the children hold the prompt
@@ -185,6 +194,7 @@ def test_forks_share_their_prompt_and_go_their_own_ways():
 @pytest.mark.gpu
 def test_forks_of_forks_and_forks_within_the_window():
     b = Bench()
+    b.layer.SHARED_MIN_TILES = 0
     b.start("a", 0, 20)                                   # nothing committed yet
     b.fork("a", "b")
     b.feed("b", 1, 1300)
@@ -201,6 +211,7 @@ def test_forks_of_forks_and_forks_within_the_window():
 @pytest.mark.gpu
 def test_compaction_growth_and_shrinking_keep_every_sequence():
     b = Bench(slots=30)
+    b.layer.SHARED_MIN_TILES = 0
     for i, n in enumerate((500, 900, 260, 700)):
         b.start(i, i, n, 128)
     b.fork(1, "f")

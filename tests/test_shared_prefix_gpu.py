@@ -181,7 +181,7 @@ def test_refusals():
                      (dict(g=_lib.K2bGeom(2, 4, 128, 32, 64, 3, 3, 2, 1)), b"n_coef_heads"), (dict(batch=0), b"batch"), (dict(n_groups=-1), b"n_groups"),
                      (dict(max_members=3), b"max_members"), (dict(n_split=0), b"n_split"), (dict(n_split=65), b"n_split"), (dict(skip=None), b"null"),
                      (dict(members=None), b"null"), (dict(scale=0.0), b"sm_scale"), (dict(scale=-1.0), b"sm_scale"), (dict(nbytes=64), b"workspace"),
-                     (dict(q=a + 4), b"16-byte"), (dict(rope_pages=0), b"rope_pages")):
+                     (dict(q=a + 4), b"16-byte"), (dict(rope_pages=0), b"rope_pages"), (dict(out=a + 8), b"16-byte")):
         assert call(**kw) == _lib.BMXK_ERR_INVALID and word in lib.bmxk_last_error(), (kw, lib.bmxk_last_error())
     # outputs are checked before anything is launched, whatever the prefixes
     for kw, word in ((dict(out=None), b"output"), (dict(dtype=1), b"out_dtype")):

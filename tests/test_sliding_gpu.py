@@ -92,8 +92,8 @@ LENS = [1500, 700, 64, 1, 191, 192, 193, 1023]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("sinks", [0, 1, 4, 128, 130, 10 ** 9])
-@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 127, 128, 129, 500, 10 ** 12])
+@pytest.mark.parametrize("sinks", [0, 1, 4, 128, 130, 10 ** 9, 2 ** 63 - 1])
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 127, 128, 129, 500, 10 ** 12, 2 ** 63 - 1])
 def test_decode_sees_the_window_and_the_sinks(window, sinks):
     from bmx_b200 import kernels as K
 
@@ -188,6 +188,19 @@ def test_prompt_rows_that_see_nothing_give_zero_and_missing_fragments_are_report
 
 
 @pytest.mark.gpu
+def test_plain_decode_takes_queries_that_begin_on_any_fp16():
+    """The plain step reads queries by words where it can and by halves where it cannot."""
+    from bmx_b200 import kernels as K
+
+    w = World(K, _dev(), [700, 1500], 10 ** 9, 0)
+    q = w.q[:, :, 0].contiguous()
+    args = (w.basis, w.table, w.n_pages, w.max_pages, w.cos, w.sin, w.k_win, w.v_win, w.tail_len, w.v_lut, w.signs, 1 / math.sqrt(D), w.ws)
+    shifted = torch.empty(q.numel() + 1, dtype=torch.float16, device=q.device)[1:].view(q.shape)
+    shifted.copy_(q)
+    assert shifted.data_ptr() % 4 == 2 and torch.equal(K.k2b_decode(w.pool, shifted, *args), K.k2b_decode(w.pool, q, *args))
+
+
+@pytest.mark.gpu
 def test_another_stream_and_a_replayed_graph():
     from bmx_b200 import kernels as K
 
@@ -270,13 +283,14 @@ def test_refusals():
     lib = _lib.lib()
     a = 4096
 
-    def decode(g, window=10, sinks=0, batch=2, max_pages=3, out=a, dtype=0, ws_bytes=1 << 30, tail_cap=256):
-        return lib.bmxk_k2b_decode_sliding(ctypes.byref(g), a, a, a, a, a, 3, a, batch, max_pages, a, a, a, a, a, tail_cap, (ctypes.c_uint32 * 4)(), a,
+    def decode(g, window=10, sinks=0, batch=2, max_pages=3, out=a, dtype=0, ws_bytes=1 << 30, tail_cap=256, q=a):
+        return lib.bmxk_k2b_decode_sliding(ctypes.byref(g), q, a, a, a, a, 3, a, batch, max_pages, a, a, a, a, a, tail_cap, (ctypes.c_uint32 * 4)(), a,
                                            0.1, window, sinks, a, ws_bytes, out, dtype, None)
 
     good = _lib.K2bGeom(2, 4, 128, 32, 64, 2, 3, 2, 1)
     for kw, word in ((dict(window=0), b"window"), (dict(window=-3), b"window"), (dict(sinks=-1), b"sinks"), (dict(batch=0), b"batch"),
-                     (dict(out=None), b"output"), (dict(dtype=1), b"out_dtype"), (dict(ws_bytes=100), b"workspace")):
+                     (dict(out=None), b"output"), (dict(dtype=1), b"out_dtype"), (dict(ws_bytes=100), b"workspace"), (dict(q=a + 2), b"16-byte"),
+                     (dict(out=a + 8), b"16-byte")):
         assert decode(good, **kw) == _lib.BMXK_ERR_INVALID and word in lib.bmxk_last_error(), (kw, lib.bmxk_last_error())
     for g in (_lib.K2bGeom(2, 4, 64, 32, 64, 2, 3, 2, 0), _lib.K2bGeom(2, 4, 128, 32, 64, 2, 3, 2, 0)):
         assert decode(g) == _lib.BMXK_ERR_INVALID and b"layout 1" in lib.bmxk_last_error()
