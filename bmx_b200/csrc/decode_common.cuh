@@ -182,8 +182,8 @@ int num_sms();
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = false, int walk = WALK_ALL);
 // tcgen05 decode kernel for layout-1 pools (k2b_decode_t5.cu); two partial records per slot (one per tile parity).  Behind a prefix kernel
 // (walk.after_prefix) it is launched as that kernel's programmatic dependent: its blocks take over SMs as the prefix blocks finish (it reads
-// nothing of theirs), and each waits for the prefix kernel's completion before it ends, so that the merge kernel, which waits for this
-// one, finds both kernels' records.
+// nothing of theirs), and one of them waits for the prefix kernel's completion before it ends, so that the merge kernel, which waits for
+// this one's, finds both kernels' records.
 int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk = WALK_ALL);
 
 }  // namespace bmxk

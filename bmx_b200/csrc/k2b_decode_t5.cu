@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
   const int f_end = min(total, f_begin + per_cta);
   const int n_tiles = f_end - f_begin;
   if (n_tiles <= 0) {
-    if constexpr (WALK == WALK_OWN) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (WALK == WALK_OWN && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
 
@@ -694,7 +694,8 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
     tc5::fence_after();
     tc5::dealloc(tmem, TM_COLS);
   }
-  if constexpr (WALK == WALK_OWN) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // one block waits for the prefix kernel, so that this grid does not complete before it; the others make room for the merge kernel's blocks
+  if (WALK == WALK_OWN && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 static size_t t5_smem_bytes(int rank, int group, int batch, int walk) {
