@@ -61,7 +61,7 @@ struct TileCursor {
 constexpr int WALK_ALL = 0, WALK_OWN = 1, WALK_SLIDING = 2;
 struct K2bWalk {
   const int32_t* skip;
-  bool after_prefix;  // WALK_OWN: the prefix kernel was launched just before on the same stream; see launch_decode_t5
+  bool after_prefix;  // WALK_OWN: the prefix kernel was launched just before on the same stream (see launch_decode_t5); without it nothing is skipped
   const int32_t* tail_len;  // WALK_SLIDING: tokens in the fp16 window, or null
   int tail_cap;
   int64_t window;
@@ -75,7 +75,7 @@ struct PageSpan {
 template <int WALK>
 __device__ __forceinline__ PageSpan page_span(const K2bWalk& w, int n_pages, int b) {
   PageSpan s = {n_pages, 0, 0, 0};
-  if constexpr (WALK == WALK_OWN) s.gap = min(max(w.skip[b], 0), n_pages);
+  if constexpr (WALK == WALK_OWN) s.gap = w.after_prefix ? min(max(w.skip[b], 0), n_pages) : 0;
   if constexpr (WALK == WALK_SLIDING) {
     const int64_t total = (int64_t)n_pages * TILE_TOKENS + (w.tail_len ? min(w.tail_len[b], w.tail_cap) : 0);
     s.first = max((int64_t)0, total - w.window);
@@ -185,5 +185,7 @@ int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = fal
 // nothing of theirs), and one of them waits for the prefix kernel's completion before it ends, so that the merge kernel, which waits for
 // this one's, finds both kernels' records.
 int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk = WALK_ALL);
+// Whether its shared memory holds the lists of so many sequences.
+int check_decode_t5(int rank, int group, int batch, int walk);
 
 }  // namespace bmxk

@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(MERGE_THREADS, GQ == 4 ? 3 : 2) k2b_merge_grou
   const int cta0 = T0 / per_cta, cta1 = (tiles_b > 0) ? (T1 - 1) / per_cta : cta0 - 1;
   const int sub_slots = p.main_grid + p.batch * g.h_kv;
   const int n_cta = max(0, cta1 - cta0 + 1), n_own = n_cta * p.n_sub;
-  const int n_pre = (WALK == WALK_OWN && p.walk.skip[b] > 0) ? p.prefix_split : 0;
+  const int n_pre = (WALK == WALK_OWN && p.walk.after_prefix && p.walk.skip[b] > 0) ? p.prefix_split : 0;
   constexpr int PARTS = 8 / GQ;  // warps per query head
   const int qi = warp % GQ, part = warp / GQ;
   float M = -INFINITY, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
@@ -920,10 +920,15 @@ static int launch_merge_group(const K2bMergeParams& mp, size_t smem, cudaStream_
   return launch_merge_kernel(k2b_merge_group_kernel<WALK, GQ>, mp, (unsigned)(mp.batch * mp.g.h_kv), smem, s, after_main);
 }
 
+static size_t group_merge_smem(int G, int tail_cap) {
+  const int gq = G <= 4 ? 4 : 8;
+  return ((size_t)gq * ((tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
+}
+
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
   const int G = mp.g.n_q_groups, gq = G <= 4 ? 4 : 8;
   if (walk != WALK_ALL) {
-    size_t gsmem = ((size_t)gq * ((mp.tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
+    size_t gsmem = group_merge_smem(G, mp.tail_cap);
     BMXK_REQUIRE(gsmem <= GROUP_MERGE_SMEM, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
     // While the page-streaming kernel drains, the blocks would pile up three to an SM on the SMs that are free already; a block that asks for
     // more shared memory keeps them apart as long as the grid is small enough to spread (256 pairs: 63 -> 60 us a step; 128 pairs 52 -> 47).
@@ -1152,6 +1157,9 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   if (bad) return bad;
   const int off = check_aligned("bmxk_k2b_decode_shared", q, basis_f16, k_tail, v_tail, workspace, out);
   if (off) return off;
+  const int large = check_decode_t5(g->rank, g->group, batch, WALK_OWN);
+  if (large) return large;
+  BMXK_REQUIRE(group_merge_smem(g->n_q_groups, tail_cap) <= GROUP_MERGE_SMEM, "bmxk_k2b_decode_shared: tail_cap=%d too large for the merge kernel", tail_cap);
   const bool prefixes = n_groups > 0 && max_members > 0 && max_pages > 0;
   float* part = reinterpret_cast<float*>((uint8_t*)workspace + (bmxk_k2b_decode_workspace_bytes(g, batch, 0) + 255) / 256 * 256);
   if (prefixes) {

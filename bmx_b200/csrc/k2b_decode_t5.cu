@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(T5_THREADS, 1) k2b_decode_t5_kernel(const K2bD
 static size_t t5_smem_bytes(int rank, int group, int batch, int walk) {
   const size_t coef = (size_t)128 * rank * 2;
   return (size_t)T5_STAGES * (coef + k2b_page_block_bytes(128, group)) + (size_t)(T5_STAGES + 2) * T5_QB_BYTES + 2 * coef +
-         sizeof(T5Smem) + (size_t)((walk == WALK_ALL ? 2 : 4) * batch + 1) * 4 + 16;
+         sizeof(T5Smem) + (size_t)((walk == WALK_ALL ? 2 : walk == WALK_OWN ? 3 : 4) * batch + 1) * 4 + 16;
 }
 
 template <int RANK, int GQ, int WALK>
@@ -739,9 +739,15 @@ static int launch_t5_walk(const K2bDecodeParams& prm, int grid, size_t smem, cud
   return g4 ? launch_t5<16, 4, WALK>(prm, grid, smem, s) : launch_t5<16, 8, WALK>(prm, grid, smem, s);
 }
 
+int check_decode_t5(int rank, int group, int batch, int walk) {
+  BMXK_REQUIRE(t5_smem_bytes(rank, group, batch, walk) <= 227 * 1024, "bmxk_k2b_decode: batch=%d too large for the tcgen05 kernel's shared memory", batch);
+  return BMXK_OK;
+}
+
 int launch_decode_t5(const K2bDecodeParams& prm, int grid, cudaStream_t s, int walk) {
   const size_t smem = t5_smem_bytes(prm.g.rank, prm.g.group, prm.batch, walk);
-  BMXK_REQUIRE(smem <= 227 * 1024, "bmxk_k2b_decode: batch=%d too large for the tcgen05 kernel's shared memory", prm.batch);
+  const int bad = check_decode_t5(prm.g.rank, prm.g.group, prm.batch, walk);
+  if (bad) return bad;
   if (walk == WALK_OWN) return launch_t5_walk<WALK_OWN>(prm, grid, smem, s);
   if (walk == WALK_SLIDING) return launch_t5_walk<WALK_SLIDING>(prm, grid, smem, s);
   return launch_t5_walk<WALK_ALL>(prm, grid, smem, s);

@@ -339,6 +339,10 @@ def k2b_prefill(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: torch.Te
 
 # ---- sliding windows and shared prefixes ----------------------------------------------------------
 
+# k2b_decode_shared keeps a list of the batch's sequences and a group's window scores in shared memory beside its tiles: batches and windows
+# up to these sizes always fit (four query heads per KV head and fewer: window capacities up to k2b_decode's).
+SHARED_MAX_BATCH, SHARED_MAX_WINDOW_G8 = 2048, 5000
+
 
 def rope_fragments(rope_cos: torch.Tensor, rope_sin: torch.Tensor, n_pages: int) -> torch.Tensor:
     """The rotation tables of the first n_pages 128-token pages in the order in which the prefill kernel reads them (int32
@@ -419,7 +423,7 @@ def k2b_decode_sliding(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, 
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_sliding", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
              page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(rope_cos), _addr(rope_sin), _addr(k_tail), _addr(v_tail), _addr(tail_len),
-             tail_cap, _addr(v_lut), _addr(signs), sm_scale, int(window), int(sinks), _addr(workspace), workspace.numel(), _addr(out),
+             tail_cap, _addr(v_lut), _addr(signs), sm_scale, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
     return out
 
@@ -438,6 +442,7 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, status):
         tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert status.numel() * status.element_size() >= 16 and status.is_contiguous()
+        assert basis_f16.dtype is torch.float16 and basis_f16.is_contiguous() and basis_f16.numel() == g.h_kv * HEAD_DIM * g.rank  # read even without pages
         rope_pages = _check_fragments(rope, 0)
         out = _check_out(out, q, (torch.float16,))
         if n_split is None:
@@ -449,7 +454,7 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         call("bmxk_k2b_prefill_sliding", ctypes.byref(g), _addr(q), n_q, int(q_pos0), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16),
              _addr(page_table), page_table.stride(0), _addr(n_pages), batch, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail),
-             _addr(v_tail), _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, int(window), int(sinks), _addr(status),
+             _addr(v_tail), _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _addr(status),
              _addr(out), int(n_split), _addr(ws), nbytes, _stream())
     return out
 

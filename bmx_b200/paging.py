@@ -183,9 +183,9 @@ class PagedK2bLayer:
         self._free_rows = list(range(max_seqs - 1, -1, -1))
         self._committed: dict[object, int] = {}
         self._tail: dict[object, int] = {}
-        self._ws: dict[int, torch.Tensor] = {}      # decode workspaces by batch size
+        self._ws: dict[tuple[int, int], torch.Tensor] = {}  # decode workspaces by batch size and stream
         self._plan: tuple | None = None             # (what it holds for, page table, page counts, window rows, prefix groups, workspace) of a step
-        self._rope_frag: torch.Tensor | None = None  # rotation tables in the prefill kernel's order, as far as prefixes reach
+        self._rope_frag: tuple | None = None        # (stream, rotation tables in the prefill kernel's order, as far as prefixes reach)
 
     # ---- bookkeeping ------------------------------------------------------------------------
     def set_basis(self, basis_f32: torch.Tensor) -> None:
@@ -294,6 +294,8 @@ class PagedK2bLayer:
     # ---- decode -----------------------------------------------------------------------------
     def _prefix_groups(self, slots: list) -> tuple[list, list]:
         """(members, prefix pages) of the sequences that begin with the same slots, where attending their prefixes once pays."""
+        if len(slots) > K.SHARED_MAX_BATCH or (self.geom.n_q_groups > 4 and self.k_win.shape[2] > K.SHARED_MAX_WINDOW_G8):
+            return [], []
         first: dict[int, list[int]] = {}
         for i, s in enumerate(slots):
             if s:
@@ -316,7 +318,10 @@ class PagedK2bLayer:
         """q (len(seqs), heads, 128) fp16: one fused decode step over those sequences, each with its own pages and window; a prefix
         that several of them share is read once."""
         n = len(seqs)
-        holds = (tuple(self._rows[s] for s in seqs), tuple(seqs), self.alloc.version, self.SHARED_MIN_TILES)
+        # what a step keeps for the next belongs to the stream it was made on: another stream's step makes its own, so that nothing is read
+        # before it is written or reused while a kernel still reads it
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        holds = (tuple(self._rows[s] for s in seqs), tuple(seqs), self.alloc.version, self.SHARED_MIN_TILES, stream)
         if self._plan is None or self._plan[0] != holds:
             slots = [self.alloc.slots(s) for s in seqs]
             counts = [len(s) for s in slots]
@@ -329,9 +334,9 @@ class PagedK2bLayer:
                 if members:
                     groups = K.PrefixGroups(self.geom, n, members, pages, self.device)
                     ws = K.decode_shared_workspace(self.geom, n, groups, self.device)
-                    if self._rope_frag is None or self._rope_frag.shape[0] < groups.max_prefix:
+                    if self._rope_frag is None or self._rope_frag[0] != stream or self._rope_frag[1].shape[0] < groups.max_prefix:
                         most = self.rope_cos.shape[0] // 128
-                        self._rope_frag = K.rope_fragments(self.rope_cos, self.rope_sin, min(most, 2 * groups.max_prefix))
+                        self._rope_frag = (stream, K.rope_fragments(self.rope_cos, self.rope_sin, min(most, 2 * groups.max_prefix)))
             self._plan = (holds, table, ints, torch.tensor(holds[0], device=self.device), groups, ws, max_pg if any(counts) else 0)
         _, table, n_pages, rows, groups, ws, max_walk = self._plan
         tail = torch.tensor([self._tail[s] for s in seqs], dtype=torch.int32).to(self.device)
@@ -340,14 +345,15 @@ class PagedK2bLayer:
         tails = (self.k_win[rows].contiguous(), self.v_win[rows].contiguous(), tail)
         last = (self.v_lut, self.signs, self.sm_scale)
         if groups is not None:
-            return K.k2b_decode_shared(self.pool, q, basis16, table, n_pages, max_walk, groups, self.rope_cos, self.rope_sin, self._rope_frag, *tails, *last,
+            return K.k2b_decode_shared(self.pool, q, basis16, table, n_pages, max_walk, groups, self.rope_cos, self.rope_sin, self._rope_frag[1], *tails, *last,
                                        ws, out=out)
-        if n not in self._ws:
-            self._ws[n] = K.decode_workspace(self.geom, n, table.shape[1], self.device)
+        if (n, stream) not in self._ws:
+            self._ws[n, stream] = K.decode_workspace(self.geom, n, table.shape[1], self.device)
+        ws = self._ws[n, stream]
         if self.sliding_window is not None:
-            return K.k2b_decode_sliding(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, self._ws[n],
+            return K.k2b_decode_sliding(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, ws,
                                         self.sliding_window, self.sinks, out=out)
-        return K.k2b_decode(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, self._ws[n], out=out)
+        return K.k2b_decode(self.pool, q, basis16, table, n_pages, max_walk, self.rope_cos, self.rope_sin, *tails, *last, ws, out=out)
 
     # ---- accounting -------------------------------------------------------------------------
     def bytes_per_slot(self) -> int:

@@ -165,9 +165,11 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
  * pages are shared out over n_split CTAs; the pages behind it, the fp16 window and the merge are those of bmxk_k2b_decode, whose
  * arguments and result these are (no pos_offset, no partial states).  skip, members, groups: int32 device arrays; max_members: the
  * largest group.  rope_frag: bmxk_k2b_rope_fragments of rope_pages pages (every prefix has to lie within, see the status word (3,
- * rope_pages, pages)), or null: the tables are read as they are, about a quarter slower.  Layout 1, sm_scale > 0.  workspace:
- * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once; alignment and concurrency as above.  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every
- * sequence has a cache of its own.) */
+ * rope_pages, pages)), or null: the tables are read as they are, a step of 96 sequences in 67 instead of 60 us.  Layout 1, sm_scale > 0.  workspace:
+ * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once; alignment and concurrency as above.  Refused before
+ * anything is launched: batches above what the page-streaming kernel's shared memory holds lists for (2048 always fit) and tail_cap above
+ * that of the merge (5000 always fits).  A sequence that holds nothing gives 0.  (No counterpart in bmx, where every sequence has a cache
+ * of its own.) */
 size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split);
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
                            const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
@@ -222,7 +224,8 @@ int bmxk_k2b_rope_fragments(const void* rope_cos, const void* rope_sin, int n_pa
 /* bmxk_k2b_prefill_split under a sliding window with sinks: query row i at position x = q_pos0 + i sees the keys at positions in (x - window, x]
  * and those < min(sinks, x + 1).  Pages that no row sees are not read and their page-table entries may be anything.  rope_frag: see
  * bmxk_k2b_rope_fragments (every page that a row's position reaches has to lie within rope_pages), or null.  q and out 16-byte
- * aligned, sm_scale > 0.  A row that sees nothing gives 0. */
+ * aligned, sm_scale > 0.  A row that sees nothing gives 0.  What no row of a block of 128 / n_q_groups positions sees may be anything; a window
+ * value that some rows of the block see is multiplied by 0 for the others, so it has to be finite. */
 int bmxk_k2b_prefill_sliding(const bmxk_k2b_geom* g, const void* q, int n_q, int64_t q_pos0, const void* pages, const void* coefs,
                              const void* basis_f16, const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch,
                              const void* rope_cos, const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail,
