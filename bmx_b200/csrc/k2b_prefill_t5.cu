@@ -2,7 +2,7 @@
 //
 // Same job and same grid as the mma.sync kernel of k2b_prefill.cu: one CTA owns 128 / G consecutive query positions
 // of one (sequence, KV head) -- 128 attention rows with the G query heads -- and walks the visible 128-token pages and
-// then the fp16 window.  Here the three contractions of a tile are tcgen05.mma instructions issued by three warps, the
+// then the fp16 window.  Here the three contractions of a tile are tcgen05.mma instructions issued by a warp each, the
 // attention rows live on the 128 lanes of tensor memory (one softmax thread per row: no reduction across threads),
 // and the dequantization of tile n+1 runs in its own warps while tile n is multiplied and normalised:
 //
@@ -13,9 +13,8 @@
 //                                  Two more "channels" carry log2(value norm) / scale as an fp16 pair (high part,
 //                                  remainder) against two ones in Q, so that the scores arrive with the norm in the
 //                                  exponent and the weights leave the softmax as p * norm with ONE rounding to fp16
-//   U2  S[128 rows x 64 tok]     = Q (smem) x K^T over 144 channels, fp32, once per half of the tile: the two halves
-//                                  have their own score and weight columns, so U2 of one half runs while the other
-//                                  half is in the softmax
+//   U2  S[128 rows x 128 tok]    = Q (smem) x K^T over 144 channels, fp32, once per tile; each half of its score columns has a set of softmax
+//                                  warps and weight columns of its own
 //   softmax warps (2 x 4; thread = row, one set per half): running maximum (base 2) by turns; only when a score exceeds it
 //                                  by more than 8 does it move and the accumulator get rescaled;
 //                                  weights -> tensor memory as fp16 (A operand of U3)
@@ -33,6 +32,16 @@
 // Few query rows against a long context leave most SMs idle and one CTA with the whole page walk: with n_split > 1 the
 // visible pages of a block are shared out over n_split CTAs, each writes a partial record per row (accumulators after
 // the rotation is undone, running maximum, sum of weights) and a small kernel merges them.
+//
+// The kernel serves three kinds of rows (MODE): the positions of a causal prompt; those of a prompt under a sliding window with sinks, whose
+// block walks the sinks' pages and those from its first row's window on (a row's own edges are the causal mask's second bound); and the
+// single-token queries of up to 128 / G sequences over the prefix of pages they share, which is dequantized once for all of them and left as
+// partial records for the merge of a decode step.
+//
+// What bounds it: about 2800 cycles per tile and CTA where the floor of its three contractions is 1100 -- the chain key dequantization ->
+// U2 -> softmax -> U3 with 28 warps at 60 % of the issue slots (tensor pipe 40 %, exponentials 33 %) -- and 5.6 us before the first and after the
+// last tile.  Measured: 128 sequences x 8 heads behind 128 shared pages 62 us, 2 x 2048 rows under a window of 2048 311 us, 512 causal rows over 16k
+// tokens 247 us.
 //
 // Every wait is bounded and reports through the status words; nothing here waits on another CTA.
 #include <type_traits>
@@ -69,6 +78,7 @@ struct P5Smem {
   uint64_t keys[2], klow;                      // key warps (8): keys of the tile written [tile parity]; K_low in registers (U1 of the next may start)
   uint64_t values[2], scores[2], weights[2];   // per half (4 warps): value operand written, scores read, weights written
   uint64_t turn[2][4];                         // [half][group of 32 rows]: the half's running maximum is settled (the two warps of a group alternate)
+  uint64_t ready;                              // Q laid out (16 warps)
   uint64_t rot[4];                             // steps of the inverse value rotation that both warps of a group are through
   uint32_t tmem_base;
   float m[128];  // the running maximum of each row, valid for the halves settled so far
@@ -97,6 +107,10 @@ __device__ __forceinline__ bool elect_one_p5() {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* status, int where) {
   return __all_sync(0xffffffffu, wait_or_flag(bar, parity, status, where) ? 1 : 0) != 0;
 }
+
+// An operand `off` 16-byte units behind that of a descriptor: the address is in its low half and does not carry into the high one (64-bit
+// sums cost the issuing warps twice the registers, and spills in front of every product).
+__device__ __forceinline__ uint64_t desc_at(uint64_t d, int off) { return (d & 0xFFFFFFFF00000000ull) | (uint32_t)((uint32_t)d + (uint32_t)off); }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   uint32_t r;
@@ -138,18 +152,47 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
   // no 64-bit arithmetic in what every thread runs here: it was half of the time to the first tile.
   auto head_of = [&](int m) { return MODE == MODE_PREFIX ? m - (int)((uint32_t)(m * p.g_inv) >> 10) * G : m >> p.pp_log; };
   auto pos_of = [&](int m) { return MODE == MODE_PREFIX ? (int)((uint32_t)(m * p.g_inv) >> 10) : m & (PP - 1); };
-  // The operands that do not change are fetched ahead: what follows waits for the page counts first (a load of memory that the SM has not
-  // touched takes 1 - 2 us).  One line per thread.  (A block under a sliding window is short: 2 x 2048 rows 343 -> 338 us.  Long ones gain nothing.)
-  if constexpr (MODE == MODE_SLIDING) {
-    const uint8_t* basis = reinterpret_cast<const uint8_t*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK);
-    const uint8_t* at = nullptr;
-    if (tid < COEF_BYTES / 128) at = basis + tid * 128;
-    else if (tid >= 128 && tid < 132) at = reinterpret_cast<const uint8_t*>(p.signs) + (tid - 128) * 128;
-    else if (tid >= 256 && tid < 512) {
-      const int m = (tid - 256) >> 1;
-      at = reinterpret_cast<const uint8_t*>(p.q + (((int64_t)b * H + h * G + head_of(m)) * p.n_q + min(i0 + pos_of(m), p.n_q - 1)) * HEAD_DIM) + ((tid & 1) << 7);
+  // ---- prologue: the operands that do not change (Q, basis, constant rows of V'), barriers, tensor memory ----
+  // Q belongs to the softmax and value warps and only U2 waits for it (sh->ready), the rest to the key warps, barriers and the first copies to
+  // warp 16, tensor memory to warp 17.  Loads of memory that the SM has not touched take 1 - 2 us: those whose addresses do not depend on the
+  // page counts and groups are issued before these are waited for.  (Against one layout by all warps behind the geometry and before one barrier:
+  // 32 sequences behind 64 pages 56.2 -> 54.9 us a step, 2 x 2048 rows under a window of 2048 316 -> 311.)
+  const bool q_warp = (warp >= 8 && warp < 16) || warp >= 20;
+  const int qt = tid - (warp < 16 ? 256 : 384);  // of the 512 threads that lay out Q
+  uint4 qv[4];
+  if (MODE != MODE_PREFIX && q_warp) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // 16 bytes c8 of row m
+      const int m = (qt >> 4) + 32 * i, c8 = qt & 15;
+      qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (((int64_t)b * H + h * G + head_of(m)) * p.n_q + min(i0 + pos_of(m), p.n_q - 1)) * HEAD_DIM) + c8);
     }
-    if (at) asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+  }
+  auto write_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = (qt >> 4) + 32 * i, c8 = qt & 15;
+      *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = qv[i];
+    }
+  };
+  constexpr int NB = 128 * (RANK / 8) / 256;
+  uint4 bv[NB];
+  float sv = 0.f;
+  if (warp < 8) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) bv[i] = __ldg(reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK) + tid + 256 * i);
+    if (tid < 128) sv = __ldg(p.signs + tid);
+  }
+  if (warp == 16 && lane == 0) {
+    for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 16);
+    mbar_init(&sh->low, 1), mbar_init(&sh->klow, 8), mbar_init(&sh->ready, 16);
+    for (int e = 0; e < 2; ++e) {
+      mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1), mbar_init(&sh->keys[e], 8);
+      mbar_init(&sh->values[e], 4), mbar_init(&sh->scores[e], 4), mbar_init(&sh->weights[e], 4);
+      for (int w = 0; w < 4; ++w) mbar_init(&sh->turn[e][w], 1);
+    }
+    for (int w = 0; w < 4; ++w) mbar_init(&sh->rot[w], 2);
+    fence_barrier_init();
+    fence_proxy_async();
   }
   const int4 group = MODE == MODE_PREFIX ? reinterpret_cast<const int4*>(p.groups)[b] : make_int4(0, 0, b, 0);
   const int m0 = group.x, n_members = group.y - group.x, first_member = group.z;
@@ -186,20 +229,16 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     bulk_g2s(st + COEF_BYTES, p.pages + ((int64_t)slot * g.h_kv + h) * PB, PB, &sh->full[stage]);
   };
 
-  // ---- prologue: barriers, tensor memory, the operands that do not change (Q, basis, constant rows of V') ----
-  // (warp 16: barriers and the first copies; the others: the operands; warp 17 also tensor memory)
+  if (MODE == MODE_PREFIX && q_warp) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = (qt >> 4) + 32 * i;
+      const int seq = __ldg(p.members + m0 + min(i0 + pos_of(m), n_members - 1));
+      qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q) + (uint32_t)((seq * H + h * G + head_of(m)) * 16 + (qt & 15)));
+    }
+  }
   if (warp == 16) {
     if (lane == 0) {
-      for (int s = 0; s < P5_STAGES; ++s) mbar_init(&sh->full[s], 1), mbar_init(&sh->empty[s], 16);
-      mbar_init(&sh->low, 1), mbar_init(&sh->klow, 8);
-      for (int e = 0; e < 2; ++e) {
-        mbar_init(&sh->sdone[0][e], 1), mbar_init(&sh->sdone[1][e], 1), mbar_init(&sh->odone[e], 1), mbar_init(&sh->keys[e], 8);
-        mbar_init(&sh->values[e], 4), mbar_init(&sh->scores[e], 4), mbar_init(&sh->weights[e], 4);
-        for (int w = 0; w < 4; ++w) mbar_init(&sh->turn[e][w], 1);
-      }
-      for (int w = 0; w < 4; ++w) mbar_init(&sh->rot[w], 2);
-      fence_barrier_init();
-      fence_proxy_async();
       // the first tiles travel while the operands that do not change are laid out
       int slot[P5_STAGES];
 #pragma unroll
@@ -209,54 +248,42 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         if (s < NP) copy_tile(s, slot[s]);
     }
     __syncwarp();
-  } else {
-    // every load of a thread is in flight before its first store
-    constexpr int ST = P5_THREADS - 32, NQ = (128 * 16 + ST - 1) / ST;
-    const int st = tid - (warp > 16 ? 32 : 0);
-    if (warp == 17) {
-      tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
-      tc5::relinquish();
-    }
-    uint4 qv[NQ];
+  } else if (warp == 17) {
+    tc5::alloc(smem_u32(&sh->tmem_base), TM_COLS);
+    tc5::relinquish();
+  } else if (MODE != MODE_PREFIX && q_warp) {
+    write_q();
+    fence_proxy_async();
+  } else if (warp < 8) {
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {  // 16 bytes c8 of row m
-      const int o = st + i * ST, m = o >> 4, c8 = o & 15;
-      if (m < 128) {
-        const int64_t qrow = MODE == MODE_PREFIX ? (int64_t)__ldg(p.members + m0 + min(i0 + pos_of(m), n_members - 1)) * H + h * G + head_of(m)
-                                                 : ((int64_t)b * H + h * G + head_of(m)) * p.n_q + min(i0 + pos_of(m), p.n_q - 1);
-        qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q + qrow * HEAD_DIM) + c8);
-      }
+    for (int i = 0; i < NB; ++i) {
+      const int o = tid + 256 * i, c = o / (RANK / 8), i8 = o % (RANK / 8);
+      reinterpret_cast<uint4*>(bop)[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bv[i];
     }
-    const uint4 bv = st < 128 * (RANK / 8) ? __ldg(reinterpret_cast<const uint4*>(p.basis16 + (int64_t)h * HEAD_DIM * RANK) + st) : make_uint4(0u, 0u, 0u, 0u);
-    static_assert(128 * (32 / 8) <= ST, "one piece of the basis per thread");
-    const float sv = st < 128 ? __ldg(p.signs + st) : 0.f;
-    if (st < 128) {  // K index 128, 129 of Q: ones against the norm pair; 130 .. 143 of Q and 136 .. 143 of both key buffers: zero for good
-      const int at = (st >> 3) * OP_SBO + (st & 7) * 16;
+    if (tid < 128) {  // K index 128, 129 of Q: ones against the norm pair; 130 .. 143 of Q and 136 .. 143 of both key buffers: zero for good
+      const int at = (tid >> 3) * OP_SBO + (tid & 7) * 16;
       *reinterpret_cast<uint4*>(qop + at + 16 * 128) = make_uint4(0x3C003C00u, 0u, 0u, 0u);
       *reinterpret_cast<uint4*>(qop + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
       *reinterpret_cast<uint4*>(kop0 + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
       *reinterpret_cast<uint4*>(kop0 + OP_BYTES + at + 17 * 128) = make_uint4(0u, 0u, 0u, 0u);
+      sg[tid] = sv * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
     }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int o = st + i * ST, m = o >> 4, c8 = o & 15;
-      if (m < 128) *reinterpret_cast<uint4*>(qop + (m >> 3) * OP_SBO + c8 * 128 + (m & 7) * 16) = qv[i];
-    }
-    if (st < 128 * (RANK / 8)) {
-      const int c = st / (RANK / 8), i8 = st % (RANK / 8);
-      reinterpret_cast<uint4*>(bop)[((c >> 3) * (RANK / 8) + i8) * 8 + (c & 7)] = bv;
-    }
-    if (st < 16 * 16) {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
-      const int r = 128 + (st >> 4), i = st & 15;
+    {  // rows 128 .. 143: 1/norm pair (rewritten per tile), ones, zeros
+      const int r = 128 + (tid >> 4), i = tid & 15;
       const uint32_t w = (r == 130) ? 0x3C003C00u : 0u;
       *reinterpret_cast<uint4*>(vop + (r >> 3) * V_SBO + i * 128 + (r & 7) * 16) = make_uint4(w, w, w, w);
     }
-    if (st < 128) sg[st] = sv * (1.0f / 128.0f);  // signs * fwht / sqrt(d), with the orthonormal fwht = butterflies / sqrt(d)
+    fence_proxy_async();
   }
-  fence_proxy_async();
   tc5::fence_before();
   __syncthreads();
   tc5::fence_after();
+  if (MODE == MODE_PREFIX && q_warp) {
+    write_q();
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh->ready);
+  }
   const uint32_t tmem = sh->tmem_base;
 
   if (warp < 8) {
@@ -480,8 +507,6 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     const uint32_t tl_ = tmem + ((uint32_t)(32 * wq) << 16);
     const int qi = head_of(row), ip = i0 + pos_of(row);
     const int x = p.q_rel + ip, win = MODE == MODE_SLIDING ? x - p.window + 1 : 0;  // this row's position, the first of its window
-    const bool in_group = MODE == MODE_PREFIX && row < PP * G && ip < n_members;
-    const int my_seq = in_group ? p.members[m0 + ip] : 0;  // for the record at the end
     float m = -1e30f;
     bool alive = true;
 
@@ -654,6 +679,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     }
     PROF_OUT(48, 8)
     // ---- the last U3, the rotation if no window tile undid it, normalise and store: each set takes 64 of the channels ----
+    const bool in_group = MODE == MODE_PREFIX && row < PP * G && ip < n_members;
+    const int my_seq = in_group ? p.members[m0 + ip] : 0;  // for the record
     if (alive && NT > 0) {
       alive = warp_wait(&sh->turn[1][wq], (uint32_t)(NT - 1) & 1u, p.status, 54);  // the last half is settled
       m = sh->m[row];
@@ -672,8 +699,9 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
     }
     if (alive) {
       // A row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used) and leave
-      // whole lines at a time.  (16 bytes of 32 rows per store kept the store unit busy for 2 us.)
-      uint4* stage = reinterpret_cast<uint4*>(kop0) + (warp - 8) * 32 * 17;
+      // whole lines at a time.  (16 bytes of 32 rows per store kept the store unit busy for 2 us.)  The space begins with the raw stages: an
+      // operand's address, held through the loop for this, was spilled by every role (512 causal rows over 16k tokens 251 -> 247 us).
+      uint4* stage = reinterpret_cast<uint4*>(smem) + (warp - 8) * 32 * 17;
       auto rows_out = [&](auto n16_, uint64_t to) {  // n16 16-byte pieces per row, row r to the address that lane r holds (0: nowhere)
         constexpr int n16 = decltype(n16_)::value;
         __syncwarp();
@@ -753,9 +781,9 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         if (n >= 1 && !warp_wait(&sh->klow, (uint32_t)(n - 1) & 1u, p.status, 57)) break;
         tc5::fence_after();
         if (el) {
-          const uint64_t da = d_stage + (uint64_t)(s * (STAGE_BYTES >> 4));
+          const uint64_t da = desc_at(d_stage, s * (STAGE_BYTES >> 4));
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) tc5::mma_ss(tmem + TM_KL, da + 16 * ks, d_b + 16 * ks, ID_U1, ks > 0);
+          for (int ks = 0; ks < KS; ++ks) tc5::mma_ss(tmem + TM_KL, desc_at(da, 16 * ks), desc_at(d_b, 16 * ks), ID_U1, ks > 0);
           tc5::commit(smem_u32(&sh->low));
         }
         __syncwarp();
@@ -766,14 +794,15 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       // made U2 wait for shared memory); each half's softmax warps have a barrier of their own
       constexpr uint32_t ID_U2 = tc5::idesc_f16_f32(128, 128);
       const uint64_t d_q = tc5::smem_desc(smem_u32(qop), 128, OP_SBO), d_k = tc5::smem_desc(smem_u32(kop0), 128, OP_SBO);
-      for (int n = 0; n < NT; ++n) {
+      const bool ready = MODE != MODE_PREFIX || warp_wait(&sh->ready, 0u, p.status, 61);
+      for (int n = 0; n < NT && ready; ++n) {
         if (n >= 1 && !(warp_wait(&sh->scores[0], (uint32_t)(n - 1) & 1u, p.status, 51) && warp_wait(&sh->scores[1], (uint32_t)(n - 1) & 1u, p.status, 51))) break;
         if (!warp_wait(&sh->keys[n & 1], (uint32_t)(n >> 1) & 1u, p.status, 58)) break;
         tc5::fence_after();
         if (el) {
-          const uint64_t db = d_k + (uint64_t)((n & 1) * (OP_BYTES >> 4));
+          const uint64_t db = desc_at(d_k, (n & 1) * (OP_BYTES >> 4));
 #pragma unroll
-          for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S, d_q + 16 * ks, db + 16 * ks, ID_U2, ks > 0);  // 144 channels
+          for (int ks = 0; ks < 9; ++ks) tc5::mma_ss(tmem + TM_S, desc_at(d_q, 16 * ks), desc_at(db, 16 * ks), ID_U2, ks > 0);  // 144 channels
           tc5::commit(smem_u32(&sh->sdone[0][n & 1]));
           tc5::commit(smem_u32(&sh->sdone[1][n & 1]));
         }
@@ -790,7 +819,7 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
         if (el) {
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)  // 64 tokens of the half: weight columns 32 hf .., token chunks 8 hf ..
-            tc5::mma_ts(tmem + TM_O, tmem + TM_P + 32 * hf + 8 * ks, d_v + 64 * hf + 16 * ks, ID_U3, (u > 0 || ks > 0) ? 1u : 0u);
+            tc5::mma_ts(tmem + TM_O, tmem + TM_P + 32 * hf + 8 * ks, desc_at(d_v, 64 * hf + 16 * ks), ID_U3, (u > 0 || ks > 0) ? 1u : 0u);
           tc5::commit(smem_u32(&sh->odone[hf]));
         }
         __syncwarp();
