@@ -634,8 +634,9 @@ __global__ void __launch_bounds__(MERGE_THREADS, 2) k2b_merge_kernel(const K2bMe
 // ---------------------------------------------------------------------------------------------
 // Merge of a step under a sliding window or behind shared prefixes: one block of 256 threads per (sequence, KV head) serves all its query
 // heads, so that a window row is read and widened once for the group (the kernel above reads it once per query head).  Against a variant
-// of that kernel, in a step of 128 sequences x 8 KV heads x 4 query heads with 4 prefix records each: 87 -> 35 us; 32 sequences with 18
-// records 26 -> 10 us; one sequence: the same time.
+// of that kernel, in a step of 128 sequences x 8 KV heads x 4 query heads with 4 prefix records each: 87 -> 27 us by itself (18 us of a step,
+// which it enters while the page-streaming kernel drains); 32 sequences with 18 records 26 -> 10 us; one sequence: the same time.  Bound by
+// instruction issue (54 %) and the latency of one wave of blocks, not by the 63 MB that it reads there (0.29 of the DRAM rate).
 //   scores   mma.sync over 16 tokens and eight queries per warp; operands straight from global memory, the channels taken in an order
 //            in which a lane's eight are one 16-byte piece (the order of a contraction is free)
 //   values   thread = (channel octet, token group of 16), GQ x 8 accumulators; every row is loaded once

@@ -38,9 +38,9 @@
 // single-token queries of up to 128 / G sequences over the prefix of pages they share, which is dequantized once for all of them and left as
 // partial records for the merge of a decode step.
 //
-// What bounds it: about 2800 cycles per tile and CTA where the floor of its three contractions is 1100 -- the chain key dequantization ->
-// U2 -> softmax -> U3 with 28 warps at 60 % of the issue slots (tensor pipe 40 %, exponentials 33 %) -- and 5.6 us before the first and after the
-// last tile.  Measured: 128 sequences x 8 heads behind 128 shared pages 62 us, 2 x 2048 rows under a window of 2048 311 us, 512 causal rows over 16k
+// What bounds it: about 2800 cycles per tile and CTA, 1100 of them with the tensor pipe at work -- the chain key dequantization -> U2 -> softmax
+// -> U3, 28 warps at 60 % of the issue slots (tensor pipe 40 %, exponentials 33 %) -- and about 10 us before the first tile's keys and after the
+// last one's.  Measured: 128 sequences x 8 heads behind 128 shared pages 62 us, 2 x 2048 rows under a window of 2048 311 us, 512 causal rows over 16k
 // tokens 247 us.
 //
 // Every wait is bounded and reports through the status words; nothing here waits on another CTA.

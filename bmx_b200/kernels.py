@@ -376,29 +376,35 @@ def split_walk(ctas: int, pages: int, device, most: int = 64) -> int:
 
 def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int, basis_f16: torch.Tensor | None,
                 rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, k_tail: torch.Tensor | None, v_tail: torch.Tensor | None,
-                tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor) -> int:
-    """What every step over a k2b pool asks of its tensors; returns the window's capacity."""
+                tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor) -> tuple[int, int, int]:
+    """What every step over a k2b pool asks of its tensors; returns the batch, the page table's row stride and the window's capacity.
+    (Every look at a tensor costs 50 - 250 ns, as much as the call's argument conversion in all: shapes and strides are read once.)"""
     g = pool.geom
-    h_kv, batch, half, i32 = g.h_kv, q.shape[0], torch.float16, torch.int32
-    assert q.dtype is half and q.is_contiguous() and q.shape[1] == h_kv * g.n_q_groups and q.shape[-1] == HEAD_DIM
+    h_kv, half, i32 = g.h_kv, torch.float16, torch.int32
+    shape = q.shape
+    batch = shape[0]
+    assert q.dtype is half and q.is_contiguous() and shape[1] == h_kv * g.n_q_groups and shape[-1] == HEAD_DIM
     rows, columns = page_table.shape
-    assert page_table.dtype is i32 and rows == batch and page_table.stride(1) == 1
+    stride, unit = page_table.stride()
+    assert page_table.dtype is i32 and rows == batch and unit == 1
     assert n_pages.dtype is i32 and n_pages.shape == (batch,) and n_pages.is_contiguous()
     assert 0 <= max_pages <= columns, f"max_pages={max_pages}: the page table has {columns} columns"
     assert signs.dtype is torch.float32 and signs.numel() == HEAD_DIM and signs.is_contiguous()
     assert v_lut.dtype is i32 and v_lut.numel() == 4 and not v_lut.is_cuda, "v_lut: v_lut_tensor(), on the host"
     if max_pages > 0:
         assert basis_f16.dtype is half and basis_f16.is_contiguous() and basis_f16.numel() == h_kv * HEAD_DIM * g.rank
-        for t in (rope_cos, rope_sin):
-            assert t.dtype is half and t.is_contiguous() and t.shape[1] == HEAD_DIM and t.shape[0] >= 128
+        positions, dim = rope_cos.shape
+        assert rope_cos.dtype is half and rope_cos.is_contiguous() and dim == HEAD_DIM and positions >= 128
+        positions, dim = rope_sin.shape
+        assert rope_sin.dtype is half and rope_sin.is_contiguous() and dim == HEAD_DIM and positions >= 128
     if k_tail is None:
         assert v_tail is None and tail_len is None
-        return 0
+        return batch, stride, 0
     shape = k_tail.shape
     assert k_tail.dtype is half and v_tail.dtype is half and k_tail.is_contiguous() and v_tail.is_contiguous()
     assert shape == (batch, h_kv, shape[2], HEAD_DIM) and v_tail.shape == shape
     assert tail_len.dtype is i32 and tail_len.shape == (batch,) and tail_len.is_contiguous()
-    return shape[2]
+    return batch, stride, shape[2]
 
 
 def _check_out(out: torch.Tensor | None, q: torch.Tensor, dtypes: tuple) -> torch.Tensor:
@@ -419,10 +425,10 @@ def k2b_decode_sliding(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, 
     g = pool.geom
     assert q.dim() == 3
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, signs, workspace):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
+        batch, stride, tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_sliding", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
-             page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(rope_cos), _addr(rope_sin), _addr(k_tail), _addr(v_tail), _addr(tail_len),
+             stride, _addr(n_pages), batch, max_pages, _addr(rope_cos), _addr(rope_sin), _addr(k_tail), _addr(v_tail), _addr(tail_len),
              tail_cap, _addr(v_lut), _addr(signs), sm_scale, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
     return out
@@ -434,13 +440,14 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
                         status: torch.Tensor, window: int, sinks: int = 0, out: torch.Tensor | None = None, n_split: int | None = None) -> torch.Tensor:
     """k2b_prefill under a sliding window: row i of q (batch, heads, n_q, 128) fp16 stands at position x = q_pos0 + i and sees the
     keys in (x - window, x] and the first `sinks` up to x.  Pages that no row sees are not read.  rope: rope_fragments() of every page held
-    up to the last row's position (too few are reported in the status word), or None (the tables are read as they are).  status: zeroed device memory (a decode workspace serves).  n_split: shares of
-    a block's page walk, by default what fills the GPU."""
+    up to the last row's position (too few are reported in the status word), or None (the tables are read as they are).  status: zeroed
+    device memory (a decode workspace serves).  n_split: shares of a block's page walk, by default what fills the GPU.  A window row that
+    some query of a block of 128 // n_q_groups positions sees has to hold finite values."""
     g = pool.geom
     assert q.dim() == 4 and q.shape[2] >= 1
-    batch, n_q = q.shape[0], q.shape[2]
+    n_q = q.shape[2]
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, status):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
+        batch, stride, tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert status.numel() * status.element_size() >= 16 and status.is_contiguous()
         assert basis_f16.dtype is torch.float16 and basis_f16.is_contiguous() and basis_f16.numel() == g.h_kv * HEAD_DIM * g.rank  # read even without pages
         rope_pages = _check_fragments(rope, 0)
@@ -453,7 +460,7 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
         nbytes = int(_lib.lib().bmxk_k2b_prefill_workspace_bytes(ctypes.byref(g), n_q, batch, int(n_split)))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         call("bmxk_k2b_prefill_sliding", ctypes.byref(g), _addr(q), n_q, int(q_pos0), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16),
-             _addr(page_table), page_table.stride(0), _addr(n_pages), batch, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail),
+             _addr(page_table), stride, _addr(n_pages), batch, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail),
              _addr(v_tail), _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, min(int(window), 1 << 40), min(int(sinks), 1 << 40), _addr(status),
              _addr(out), int(n_split), _addr(ws), nbytes, _stream())
     return out
@@ -511,12 +518,12 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
     assert q.dim() == 3 and groups.batch == q.shape[0], f"groups of a batch of {groups.batch}, queries of {q.shape[0]}"
     with _on_device_of(q, pool.pages, pool.coefs, page_table, n_pages, basis_f16, rope_cos, rope_sin, rope, k_tail, v_tail, tail_len, signs, workspace,
                        groups.skip):
-        tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
+        batch, stride, tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
         rope_pages = _check_fragments(rope, groups.max_prefix)
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_shared", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
-             page_table.stride(0), _addr(n_pages), q.shape[0], max_pages, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
+             stride, _addr(n_pages), batch, max_pages, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
              groups.n_groups, groups.max_members, groups.n_split, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail), _addr(v_tail),
              _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
