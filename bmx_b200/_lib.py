@@ -135,7 +135,7 @@ _SIGNATURES = {
                                          c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float,
                                          c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "bmxk_k2b_decode_shared_workspace_bytes": (c_size_t, [POINTER(K2bGeom), c_int, c_int]),
-    "bmxk_k2b_decode_shared": (c_int, [POINTER(K2bGeom), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+    "bmxk_k2b_decode_shared": (c_int, [POINTER(K2bGeom), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p,
                                        c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                        c_int, c_void_p, c_void_p, c_float, c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
     "bmxk_copy_slots": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p]),

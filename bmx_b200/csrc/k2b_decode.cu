@@ -1091,7 +1091,7 @@ static int decode_step(const bmxk_k2b_geom* g, const void* q, const void* pages,
   mp.tail_cap = tail_cap, mp.signs = signs, mp.scale_log2 = scale_log2, mp.out = out, mp.out_dtype = out_dtype;
   mp.partial_out = partial_out;
   mp.walk = w, mp.prefix_part = prefix_part, mp.prefix_split = prefix_split;
-  return launch_merge(mp, s, walk_pages > 0 && (phases & 1), walk);
+  return launch_merge(mp, s, w.after_prefix || (walk_pages > 0 && (phases & 1)), walk);
 }
 
 extern "C" {
@@ -1134,8 +1134,8 @@ size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch,
 }
 
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
-                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
-                           const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, int max_own_pages,
+                           const int32_t* skip, const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
                            const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
                            const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
                            size_t workspace_bytes, void* out, int out_dtype, void* stream) {
@@ -1147,6 +1147,7 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   BMXK_REQUIRE(g->n_coef_heads == 1 || g->n_coef_heads == g->h_kv, "bmxk_k2b_decode_shared: n_coef_heads=%d", g->n_coef_heads);
   BMXK_REQUIRE(batch >= 1 && max_pages >= 0 && n_groups >= 0 && n_groups <= 65535 && max_members >= 0 && max_members <= batch,
                "bmxk_k2b_decode_shared: batch=%d max_pages=%d n_groups=%d max_members=%d", batch, max_pages, n_groups, max_members);
+  BMXK_REQUIRE(max_own_pages >= 0 && max_own_pages <= max_pages, "bmxk_k2b_decode_shared: max_own_pages=%d of max_pages=%d", max_own_pages, max_pages);
   BMXK_REQUIRE(n_split >= 1 && n_split <= 64, "bmxk_k2b_decode_shared: n_split=%d must be in 1..64", n_split);
   BMXK_REQUIRE(skip && (n_groups == 0 || (members && groups && ((uintptr_t)groups & 15) == 0)), "bmxk_k2b_decode_shared: null or misaligned group lists");
   BMXK_REQUIRE(sm_scale > 0.f, "bmxk_k2b_decode_shared: sm_scale=%g must be positive", sm_scale);
@@ -1187,8 +1188,8 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   K2bWalk w = {};
   w.skip = skip, w.after_prefix = prefixes;
   return decode_step(g, q, pages, coefs, basis_f16, page_table, table_stride, n_pages, batch, max_pages, rope_cos, rope_sin, 0, k_tail, v_tail,
-                     tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, nullptr, 3, WALK_OWN, w, max_pages,
-                     part, n_split, stream);
+                     tail_len, tail_cap, v_lut, signs, sm_scale, workspace, workspace_bytes, out, out_dtype, nullptr, 3, WALK_OWN, w,
+                     prefixes ? max_own_pages : max_pages, part, n_split, stream);
 }
 
 int bmxk_k2b_decode_static(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs,

@@ -494,6 +494,7 @@ class PrefixGroups:
                 skip[int(r)] = int(p)
         self.batch, self.n_groups, self.max_members = batch, len(members), max((len(m) for m in members), default=0)
         self.max_prefix = max(prefix_pages, default=0)
+        self.min_prefix = min(skip)  # over the batch: 0 with a row in no group
         packed = torch.tensor(info + skip + rows, dtype=torch.int32).to(device)
         self.info, self.skip, self.members = packed[:len(info)], packed[len(info):len(info) + batch], packed[len(info) + batch:]
         pp = 128 // g.n_q_groups
@@ -523,7 +524,7 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
         rope_pages = _check_fragments(rope, groups.max_prefix)
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_shared", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
-             stride, _addr(n_pages), batch, max_pages, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
+             stride, _addr(n_pages), batch, max_pages, max_pages - groups.min_prefix, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
              groups.n_groups, groups.max_members, groups.n_split, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail), _addr(v_tail),
              _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())

@@ -163,7 +163,8 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
  * the sequences members[begin] .. members[end - 1] (each in one group at most) have page-table rows that begin with the same `pages`
  * entries, read from the row of `first`, one of them; skip[s] = pages for them and 0 for a sequence in no group.  A group's prefix is dequantized once for 128 / n_q_groups sequences at a time and its
  * pages are shared out over n_split CTAs; the pages behind it, the fp16 window and the merge are those of bmxk_k2b_decode, whose
- * arguments and result these are (no pos_offset, no partial states).  skip, members, groups: int32 device arrays; max_members: the
+ * arguments and result these are (no pos_offset, no partial states).  max_own_pages: no sequence has more pages
+ * behind what is skipped of it (it sizes the launch that streams them; 0: none is made).  skip, members, groups: int32 device arrays; max_members: the
  * largest group.  rope_frag: bmxk_k2b_rope_fragments of rope_pages pages (every prefix has to lie within, see the status word (3,
  * rope_pages, pages)), or null: the tables are read as they are, a step of 96 sequences in 67 instead of 60 us.  Layout 1, sm_scale > 0.  workspace:
  * bmxk_k2b_decode_shared_workspace_bytes, zero-filled once; alignment and concurrency as above.  Refused before
@@ -172,8 +173,8 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
  * of its own.) */
 size_t bmxk_k2b_decode_shared_workspace_bytes(const bmxk_k2b_geom* g, int batch, int n_split);
 int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
-                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const int32_t* skip,
-                           const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
+                           const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, int max_own_pages,
+                           const int32_t* skip, const int32_t* members, const int32_t* groups, int n_groups, int max_members, int n_split, const void* rope_cos,
                            const void* rope_sin, const void* rope_frag, int rope_pages, const void* k_tail, const void* v_tail,
                            const int32_t* tail_len, int tail_cap, const uint32_t* v_lut, const float* signs, float sm_scale, void* workspace,
                            size_t workspace_bytes, void* out, int out_dtype, void* stream);

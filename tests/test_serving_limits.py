@@ -23,7 +23,7 @@ def test_a_shared_step_that_cannot_run_is_refused_before_its_first_launch():
     a = 4096
 
     def call(g, batch, tail_cap):
-        return lib.bmxk_k2b_decode_shared(ctypes.byref(g), a, a, a, a, a, 3, a, batch, 3, a, a, a, 1, 2, 1, a, a, a, 4, a, a, a, tail_cap,
+        return lib.bmxk_k2b_decode_shared(ctypes.byref(g), a, a, a, a, a, 3, a, batch, 3, 2, a, a, a, 1, 2, 1, a, a, a, 4, a, a, a, tail_cap,
                                           (ctypes.c_uint32 * 4)(), a, 0.1, a, 1 << 40, a, 0, None)
 
     assert call(_lib.K2bGeom(1, 4, 128, 32, 64, 1, 3, 2, 1), 4000, 192) == _lib.BMXK_ERR_INVALID and b"batch=4000" in lib.bmxk_last_error()

@@ -172,15 +172,15 @@ def test_refusals():
     good = _lib.K2bGeom(2, 4, 128, 32, 64, 2, 3, 2, 1)
 
     def call(g=good, q=a, batch=2, skip=a, members=a, n_groups=1, max_members=2, n_split=1, frag=a, rope_pages=4, scale=0.1, nbytes=1 << 30, out=a, dtype=0,
-             max_pages=3):
-        return lib.bmxk_k2b_decode_shared(ctypes.byref(g), q, a, a, a, a, 3, a, batch, max_pages, skip, members, a, n_groups, max_members, n_split, a, a, frag,
+             max_pages=3, own=2):
+        return lib.bmxk_k2b_decode_shared(ctypes.byref(g), q, a, a, a, a, 3, a, batch, max_pages, own, skip, members, a, n_groups, max_members, n_split, a, a, frag,
                                           rope_pages, a, a, a, 192, (ctypes.c_uint32 * 4)(), a, scale, a, nbytes, out, dtype, None)
 
     for kw, word in ((dict(g=_lib.K2bGeom(2, 4, 64, 32, 64, 2, 3, 2, 0)), b"layout 1"), (dict(g=_lib.K2bGeom(2, 9, 128, 32, 64, 2, 3, 2, 1)), b"n_q_groups"),
                      (dict(g=_lib.K2bGeom(2, 4, 128, 8, 64, 2, 3, 2, 1)), b"rank"), (dict(g=_lib.K2bGeom(2, 4, 128, 32, 48, 2, 3, 2, 1)), b"group"),
                      (dict(g=_lib.K2bGeom(2, 4, 128, 32, 64, 3, 3, 2, 1)), b"n_coef_heads"), (dict(batch=0), b"batch"), (dict(n_groups=-1), b"n_groups"),
                      (dict(max_members=3), b"max_members"), (dict(n_split=0), b"n_split"), (dict(n_split=65), b"n_split"), (dict(skip=None), b"null"),
-                     (dict(members=None), b"null"), (dict(scale=0.0), b"sm_scale"), (dict(scale=-1.0), b"sm_scale"), (dict(nbytes=64), b"workspace"),
+                     (dict(members=None), b"null"), (dict(own=-1), b"max_own_pages"), (dict(own=4), b"max_own_pages"), (dict(scale=0.0), b"sm_scale"), (dict(scale=-1.0), b"sm_scale"), (dict(nbytes=64), b"workspace"),
                      (dict(q=a + 4), b"16-byte"), (dict(rope_pages=0), b"rope_pages"), (dict(out=a + 8), b"16-byte")):
         assert call(**kw) == _lib.BMXK_ERR_INVALID and word in lib.bmxk_last_error(), (kw, lib.bmxk_last_error())
     # outputs are checked before anything is launched, whatever the prefixes
