@@ -374,6 +374,27 @@ def split_walk(ctas: int, pages: int, device, most: int = 64) -> int:
     return best
 
 
+def split_beside(ctas: int, pages: int, most: int, own_tiles: int, device) -> int:
+    """Shares (at most `most`) of a shared prefix of `pages` pages that `ctas` CTAs would each walk whole, where own_tiles tiles behind the
+    prefixes are streamed by a second kernel: it starts on the SMs that the first one leaves free, 5 us after it, and a CTA that finds
+    none runs when the first is through.  The number that makes the end of both soonest, with 10 us + 1.45 us per tile for a CTA of the first and
+    7 us + 0.85 us for one of the second (measured; over 28 steps of 4 to 128 sequences it is 2 % from the best number, split_walk's 6 %).  Against split_walk's number, a step of 32 sequences x 8 heads behind 256 pages with
+    up to 3 of their own: 18 shares 54.0 us, 14 shares 48.8; 63 sequences x 2 heads in three groups behind 40: 10 shares 31.5, 5 shares 26.1."""
+    if own_tiles <= 0:
+        return most
+    n_sm = sm_count(torch.device(device))
+    per = -(-own_tiles // n_sm)
+    own_ctas, own_time = -(-own_tiles // per), 7 + 0.85 * per
+    best, best_end = 1, None
+    for s in range(1, most + 1):
+        waves, last = -(-ctas * s // n_sm), 10 + 1.45 * -(-pages // s)
+        fits = (waves * n_sm - ctas * s) * max(0, int((last - 5) // own_time)) >= own_ctas
+        end = waves * last + (0 if fits else own_time)
+        if best_end is None or end < best_end:
+            best, best_end = s, end
+    return best
+
+
 def _check_step(pool: K2bPool, q: torch.Tensor, page_table: torch.Tensor, n_pages: torch.Tensor, max_pages: int, basis_f16: torch.Tensor | None,
                 rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, k_tail: torch.Tensor | None, v_tail: torch.Tensor | None,
                 tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor) -> tuple[int, int, int]:
@@ -477,9 +498,11 @@ def _check_fragments(rope: torch.Tensor | None, pages: int) -> int:
 class PrefixGroups:
     """Which sequences of a batch share a prefix of whole pages, for k2b_decode_shared: members[i] lists the batch rows of group i and
     prefix_pages[i] how many of the first entries of their page-table rows are the same pages.  Rows in no group are decoded as by
-    k2b_decode.  One small host-to-device copy; the object can be used for as many steps as the grouping lasts."""
+    k2b_decode.  own_pages: pages behind the prefixes, of the whole batch, if the caller knows.  One small host-to-device copy; the object can be used
+    for as many steps as the grouping lasts."""
 
-    def __init__(self, g: K2bGeom, batch: int, members: list, prefix_pages: list, device, n_split: int | None = None):
+    def __init__(self, g: K2bGeom, batch: int, members: list, prefix_pages: list, device, n_split: int | None = None,
+                 own_pages: int | None = None):
         assert batch >= 1 and len(members) == len(prefix_pages)
         rows = [int(r) for m in members for r in m]
         if len(set(rows)) != len(rows) or any(not 0 <= r < batch for r in rows):
@@ -498,8 +521,20 @@ class PrefixGroups:
         packed = torch.tensor(info + skip + rows, dtype=torch.int32).to(device)
         self.info, self.skip, self.members = packed[:len(info)], packed[len(info):len(info) + batch], packed[len(info) + batch:]
         pp = 128 // g.n_q_groups
-        ctas = g.h_kv * sum(-(-len(m) // pp) for m, p in zip(members, prefix_pages) if p)
-        self.n_split = n_split if n_split is not None else split_walk(max(1, ctas), max(1, self.max_prefix), device)
+        self._ctas, self._h_kv, self._device = max(1, g.h_kv * sum(-(-len(m) // pp) for m, p in zip(members, prefix_pages) if p)), g.h_kv, device
+        # shares of a prefix's walk: given, or at most these (see split); the workspace has room for n_split
+        self._splits, self._own = None if n_split is not None else {}, own_pages
+        self.n_split = n_split if n_split is not None else split_walk(self._ctas, max(1, self.max_prefix), device)
+
+    def split(self, own_pages: int) -> int:
+        """Shares of a prefix's walk in a step whose sequences hold up to own_pages pages behind what they share (two fifths of that on
+        average unless the caller said)."""
+        if self._splits is None:
+            return self.n_split
+        if own_pages not in self._splits:
+            own = self._h_kv * (self._own if self._own is not None else 2 * self.batch * own_pages // 5)
+            self._splits[own_pages] = split_beside(self._ctas, max(1, self.max_prefix), self.n_split, own, self._device)
+        return self._splits[own_pages]
 
 
 def decode_shared_workspace(g: K2bGeom, batch: int, groups: PrefixGroups, device) -> torch.Tensor:
@@ -522,10 +557,11 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
         batch, stride, tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
         rope_pages = _check_fragments(rope, groups.max_prefix)
+        own = max_pages - groups.min_prefix
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_shared", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),
-             stride, _addr(n_pages), batch, max_pages, max_pages - groups.min_prefix, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
-             groups.n_groups, groups.max_members, groups.n_split, _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail), _addr(v_tail),
+             stride, _addr(n_pages), batch, max_pages, own, _addr(groups.skip), _addr(groups.members), _addr(groups.info),
+             groups.n_groups, groups.max_members, groups.split(own), _addr(rope_cos), _addr(rope_sin), _addr(rope), rope_pages, _addr(k_tail), _addr(v_tail),
              _addr(tail_len), tail_cap, _addr(v_lut), _addr(signs), sm_scale, _addr(workspace), workspace.numel(), _addr(out),
              _dtype_code(out), _stream())
     return out

@@ -332,7 +332,8 @@ class PagedK2bLayer:
             if self.sliding_window is None and self.geom.layout == 1:
                 members, pages = self._prefix_groups(slots)
                 if members:
-                    groups = K.PrefixGroups(self.geom, n, members, pages, self.device)
+                    own = sum(counts) - sum(len(m) * p for m, p in zip(members, pages))
+                    groups = K.PrefixGroups(self.geom, n, members, pages, self.device, own_pages=own)
                     ws = K.decode_shared_workspace(self.geom, n, groups, self.device)
                     if self._rope_frag is None or self._rope_frag[0] != stream or self._rope_frag[1].shape[0] < groups.max_prefix:
                         most = self.rope_cos.shape[0] // 128

@@ -137,3 +137,23 @@ def test_windows_longer_than_any_integer_of_the_device():
         out = K.k2b_prefill_sliding(st.pool, q[:, :, None].contiguous(), 899, st.basis_f16, slots, n, slots.shape[1], st.rope_cos, st.rope_sin, None, *tails,
                                     st.v_lut, st.signs, st.sm_scale, ws[:256].view(torch.int32), window, sinks)
         agree(out[:, :, 0], want)
+
+
+def test_shares_of_a_prefix_leave_room_for_the_pages_behind_it(monkeypatch):
+    from bmx_b200 import kernels as K
+
+    monkeypatch.setattr(K, "sm_count", lambda device: 148)
+    for ctas, pages in ((8, 64), (8, 256), (12, 40), (32, 128), (4, 5), (300, 9), (1, 1)):
+        most = K.split_walk(ctas, pages, "cpu")
+        assert K.split_beside(ctas, pages, most, 0, "cpu") == most
+        for own in (1, 40, 148, 900, 50000):
+            s = K.split_beside(ctas, pages, most, own, "cpu")
+            assert 1 <= s <= most
+    assert K.split_beside(8, 256, 18, 307, "cpu") * 8 <= 148 - 32
+    g = K.k2b_geom(8, 4)
+    members, given = [list(range(32))], dict(own_pages=38)
+    plan = K.PrefixGroups(g, 32, members, [256], "cpu", **given)
+    assert plan.n_split == 18 and plan.split(3) == K.split_beside(8, 256, 18, 304, "cpu") < 18
+    assert K.PrefixGroups(g, 32, members, [256], "cpu", own_pages=0).split(3) == 18
+    assert K.PrefixGroups(g, 32, members, [256], "cpu").split(0) == 18
+    assert K.PrefixGroups(g, 32, members, [256], "cpu", n_split=5).split(3) == 5
