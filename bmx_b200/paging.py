@@ -150,11 +150,12 @@ class PagedK2bLayer:
     that fall between the two are freed as sequences grow.  `compact` and `resize` close the holes that finished sequences leave.
     """
 
-    # 128-token tiles per SM that attending shared prefixes once has to save over streaming them for every sequence.  Its launch and the set-up of
-    # its blocks cost about 5 us.  Measured at 8 KV heads x 4 query heads, shared against streamed: 4 sequences x 32 pages (5.2 tiles per SM
-    # saved) 21 against 22 us, 8 x 8 pages (3.0) 19 against 18, 3 x 32 (3.5) 21 against 20, 8 x 32 (12) 21 against 28, 32 x 256 46 against 398;
-    # at 1 and 8 query heads per KV head the two meet at 4 - 5 and 3.
-    SHARED_MIN_TILES = 5
+    # 128-token tiles per SM that attending shared prefixes once has to save over streaming them for every sequence; its launch and the set-up of
+    # its blocks cost the time of about one.  Measured at 8 KV heads and up to 3 pages behind the prefixes, shared against streamed: 4 query
+    # heads per KV head, 4 sequences x 2 pages (0.3 tiles per SM saved) 15 against 13 us, 4 x 4 (0.7) 15 against 17, 8 x 4 (1.5) 15 against 19, 32 x
+    # 256 49 against 402; 1 query head, 4 x 4 (0.7) 15 against 16, 2 x 16 (0.9) 16 against 14, 3 x 16 (1.7) 16 against 15, 8 x 8 (3.0) 15 against 18; 8
+    # query heads, 4 x 1 (0.2) 16 against 18, 2 x 8 (0.4) 17 against 20.
+    SHARED_MIN_TILES = 1
 
     def __init__(self, geom, n_slots: int, max_seqs: int, recent_window: int, device, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
                  *, v_seed: int = 0, max_pages_per_seq: int = 1024, sliding_window: int | None = None, sinks: int = 0):

@@ -81,7 +81,7 @@ def test_steps_on_several_streams(kw):
     b = Bench(slots=40, **kw)
     b.start("a", 0, 900)
     b.fork("a", *range(12))
-    b.layer.SHARED_MIN_TILES = 1
+    b.layer.SHARED_MIN_TILES = 0
     side = torch.cuda.Stream()
     for i in range(6):
         seqs = ["a", *range(12)][i % 3:]
