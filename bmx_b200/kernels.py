@@ -696,15 +696,20 @@ def _slot_list(slots):
     return (held, *held.buffer_info())
 
 
-def _slot_bytes(t: torch.Tensor) -> tuple[int, int]:
-    """(bytes of one slot, bytes from slot to slot) of an array whose first dimension counts slots."""
+def _slots_of(t: torch.Tensor) -> tuple:
+    """(shape, bytes of one slot, bytes from slot to slot) of an array whose first dimension counts slots."""
     shape, strides, n = t.shape, t.stride(), 1
-    for d in range(len(shape) - 1, 0, -1):
-        if strides[d] != n and shape[d] != 1:
+    d = len(shape) - 1
+    if d < 1:
+        raise ValueError(f"copy_slots: an array of slots has at least two dimensions, not {tuple(shape)}")
+    while d > 0:
+        length = shape[d]
+        if strides[d] != n and length != 1:
             raise ValueError(f"copy_slots: the values of a slot must lie in one piece, strides {strides} for shape {tuple(shape)}")
-        n *= shape[d]
+        n *= length
+        d -= 1
     item = t.element_size()
-    return n * item, (strides[0] if shape[0] > 1 else n) * item
+    return shape, n * item, (strides[0] if shape[0] > 1 else n) * item
 
 
 def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
@@ -716,16 +721,22 @@ def copy_slots(srcs: list, dsts: list, src_slots, dst_slots) -> None:
     must not write a slot that it reads, and no slot may be written twice: both are refused, like indices out of range."""
     if len(srcs) != len(dsts) or not 1 <= len(srcs) <= 8:
         raise ValueError(f"copy_slots: {len(srcs)} sources and {len(dsts)} destinations (1 to 8 of each)")
-    n, n_src, n_dst = len(srcs), srcs[0].shape[0], dsts[0].shape[0]
-    sizes = []
+    n, n_src, n_dst, sizes = len(srcs), None, None, []
     for s, d in zip(srcs, dsts):
-        if s.dim() < 2 or d is not s and (s.dtype != d.dtype or s.shape[1:] != d.shape[1:]):
-            raise ValueError(f"copy_slots: {tuple(s.shape)} {s.dtype} cannot be copied to {tuple(d.shape)} {d.dtype}")
-        if s.shape[0] != n_src or d.shape[0] != n_dst:
-            raise ValueError("copy_slots: arrays of one call have the same number of slots")
-        size, src_stride = _slot_bytes(s)
+        shape, size, src_stride = _slots_of(s)
         at = s.data_ptr()
-        sizes.append((at, at, src_stride, src_stride, size) if d is s else (at, d.data_ptr(), src_stride, _slot_bytes(d)[1], size))
+        if d is s:
+            rows, entry = shape[0], (at, at, src_stride, src_stride, size)
+        else:
+            to_shape, _, dst_stride = _slots_of(d)
+            if s.dtype != d.dtype or shape[1:] != to_shape[1:]:
+                raise ValueError(f"copy_slots: {tuple(shape)} {s.dtype} cannot be copied to {tuple(to_shape)} {d.dtype}")
+            rows, entry = to_shape[0], (at, d.data_ptr(), src_stride, dst_stride, size)
+        if n_src is None:
+            n_src, n_dst = shape[0], rows
+        elif shape[0] != n_src or rows != n_dst:
+            raise ValueError("copy_slots: arrays of one call have the same number of slots")
+        sizes.append(entry)
     a, a_at, a_n = _slot_list(src_slots)
     b, b_at, b_n = _slot_list(dst_slots)
     if a_n != b_n:
