@@ -176,7 +176,8 @@ __device__ __forceinline__ bool spin_or_flag(uint64_t* bar, uint32_t parity, int
 
 // SM count of the current device (cached) and the launcher of the merge kernel (defined in k2b_decode.cu).
 int num_sms();
-// `after_main`: the page-streaming kernel of the same step was launched just before on the same stream.  The merge
+// `after_main`: the page-streaming kernel of the same step (or, without a page behind the shared prefixes, the prefix kernel) was launched
+// just before on the same stream.  The merge
 // kernel is then launched as its programmatic dependent: its blocks may start while that kernel drains, attend over
 // the fp16 window (which that kernel does not write) and wait for it only before they read the partial states.
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main = false, int walk = WALK_ALL);

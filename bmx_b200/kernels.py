@@ -378,8 +378,9 @@ def split_beside(ctas: int, pages: int, most: int, own_tiles: int, device) -> in
     """Shares (at most `most`) of a shared prefix of `pages` pages that `ctas` CTAs would each walk whole, where own_tiles tiles behind the
     prefixes are streamed by a second kernel: it starts on the SMs that the first one leaves free, 5 us after it, and a CTA that finds
     none runs when the first is through.  The number that makes the end of both soonest, with 10 us + 1.45 us per tile for a CTA of the first and
-    7 us + 0.85 us for one of the second (measured; over 28 steps of 4 to 128 sequences it is 2 % from the best number, split_walk's 6 %).  Against split_walk's number, a step of 32 sequences x 8 heads behind 256 pages with
-    up to 3 of their own: 18 shares 54.0 us, 14 shares 48.8; 63 sequences x 2 heads in three groups behind 40: 10 shares 31.5, 5 shares 26.1."""
+    7 us + 0.85 us for one of the second (measured; over 28 steps of 4 to 128 sequences it is 2 % from the best number, split_walk's 6 %).
+    Against split_walk's number, a step of 32 sequences x 8 heads behind 256 pages with up to 3 of their own: 18 shares 54.0 us, 14 shares 48.8; 63
+    sequences x 2 heads in three groups behind 40: 10 shares 31.5, 5 shares 26.1."""
     if own_tiles <= 0:
         return most
     n_sm = sm_count(torch.device(device))

@@ -161,7 +161,8 @@ int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* p
 
 /* One decode step for sequences that share prefixes of whole pages.  groups[z] = {begin, end, first, pages} (int32 x 4, 16-byte aligned):
  * the sequences members[begin] .. members[end - 1] (each in one group at most) have page-table rows that begin with the same `pages`
- * entries, read from the row of `first`, one of them; skip[s] = pages for them and 0 for a sequence in no group.  A group's prefix is dequantized once for 128 / n_q_groups sequences at a time and its
+ * entries, read from the row of `first`, one of them; skip[s] = pages for them and 0 for a sequence in no group.  A group's prefix is
+ * dequantized once for 128 / n_q_groups sequences at a time and its
  * pages are shared out over n_split CTAs; the pages behind it, the fp16 window and the merge are those of bmxk_k2b_decode, whose
  * arguments and result these are (no pos_offset, no partial states).  max_own_pages: no sequence has more pages
  * behind what is skipped of it (it sizes the launch that streams them; 0: none is made).  skip, members, groups: int32 device arrays; max_members: the

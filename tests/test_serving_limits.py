@@ -157,3 +157,30 @@ def test_shares_of_a_prefix_leave_room_for_the_pages_behind_it(monkeypatch):
     assert K.PrefixGroups(g, 32, members, [256], "cpu", own_pages=0).split(3) == 18
     assert K.PrefixGroups(g, 32, members, [256], "cpu").split(0) == 18
     assert K.PrefixGroups(g, 32, members, [256], "cpu", n_split=5).split(3) == 5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("own", [0, 2])
+@pytest.mark.parametrize("rope", [True, False])
+def test_shared_steps_with_and_without_pages_of_their_own_replayed(own, rope):
+    """A step whose sequences hold nothing but prefix and window launches two kernels, one with more pages three: captured, replayed on other
+    queries, against the plain form."""
+    from bmx_b200 import kernels as K
+    from tests.test_shared_prefix_gpu import World, _dev
+
+    w = World(K, _dev(), [(6, [(0, 30), (own, 64), (0, 0), (0, 190)]), (3, [(own, 1), (0, 128)] * 20)], h_kv=3, G=4)
+    want = w.decode(K, rope=rope)
+    P.assert_attention(want, w.ref)
+    q, out = torch.zeros_like(w.q), torch.empty_like(w.q)
+    w.decode(K, rope=rope, q=q, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        w.decode(K, rope=rope, q=q, out=out)
+        w.decode(K, rope=rope, q=q, out=out)
+    for _ in range(3):
+        q.copy_(w.q)
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    K.check_status(w.ws)
