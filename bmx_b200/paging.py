@@ -64,7 +64,9 @@ class PageAllocator:
 
     def free(self, seq) -> int:
         """Gives back every slot of `seq`; returns how many of them nobody holds any more."""
-        return self._give_back([s for s in reversed(self._owned.pop(seq, [])) if s >= 0])
+        slots = self._owned.pop(seq, [])
+        self.version += bool(slots)  # entries of pages given back before count too: they were part of a page table
+        return self._give_back([s for s in reversed(slots) if s >= 0])
 
     def share(self, seq, other) -> list[int]:
         """`other`, which holds nothing yet, holds all slots of `seq` too (a fork: committed pages never change)."""
