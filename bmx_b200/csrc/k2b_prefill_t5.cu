@@ -685,6 +685,9 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       alive = warp_wait(&sh->turn[1][wq], (uint32_t)(NT - 1) & 1u, p.status, 54);  // the last half is settled
       m = sh->m[row];
     }
+    // A share of a prefix without tiles has no product that came after Q, which other warps lay out behind the set-up's barrier where the
+    // rows are staged below
+    if (MODE == MODE_PREFIX && NT == 0) alive = warp_wait(&sh->ready, 0u, p.status, 62);
     if (alive && NT > 0 && !(warp_wait(&sh->odone[0], (uint32_t)(NT - 1) & 1u, p.status, 49) && warp_wait(&sh->odone[1], (uint32_t)(NT - 1) & 1u, p.status, 49)))
       alive = false;
     float lsum = 0.f, add = 0.f;
@@ -698,8 +701,8 @@ __global__ void __launch_bounds__(P5_THREADS, 1) k2b_prefill_t5_kernel(const Pre
       if (MODE == MODE_PREFIX) add = p.lut_alpha * __uint_as_float(r4[2]);
     }
     if (alive) {
-      // A row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used) and leave
-      // whole lines at a time.  (16 bytes of 32 rows per store kept the store unit busy for 2 us.)  The space begins with the raw stages: an
+      // A row of a warp's 32 is a line of its own in memory: the rows pass through shared memory (every operand in it has been used, or, in a
+      // share without tiles, at least written: see above) and leave whole lines at a time.  (16 bytes of 32 rows per store kept the store unit busy for 2 us.)  The space begins with the raw stages: an
       // operand's address, held through the loop for this, was spilled by every role (512 causal rows over 16k tokens 251 -> 247 us).
       uint4* stage = reinterpret_cast<uint4*>(smem) + (warp - 8) * 32 * 17;
       auto rows_out = [&](auto n16_, uint64_t to) {  // n16 16-byte pieces per row, row r to the address that lane r holds (0: nowhere)
