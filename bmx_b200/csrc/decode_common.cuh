@@ -133,6 +133,13 @@ struct K2bDecodeParams {
 
 constexpr long long WAIT_LIMIT_CYCLES = 4000000000LL;  // ~2 s at 2 GHz
 
+// The status word says 1 once a wait of this buffer's owner ran out; every other wait then gives up too.  Other reports there (2: a full
+// window, 3: too few rearranged rotation tables) concern one call's arguments, not the waits, and do not stop the steps that follow.
+__device__ __forceinline__ bool another_gave_up(const int32_t* status) { return *reinterpret_cast<const volatile int32_t*>(status) == 1; }
+__device__ __forceinline__ void report_lost(int32_t* status, int where) {
+  if (atomicExch(status, 1) != 1) status[1] = blockIdx.x, status[2] = where;
+}
+
 __device__ __forceinline__ bool wait_or_flag(uint64_t* bar, uint32_t parity, int32_t* status, int where,
                                              long long limit = WAIT_LIMIT_CYCLES) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -142,32 +149,9 @@ __device__ __forceinline__ bool wait_or_flag(uint64_t* bar, uint32_t parity, int
   for (uint32_t spin = 1;; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((spin & 255u) == 0u) {
-      if (*reinterpret_cast<volatile int32_t*>(status) != 0) return false;  // another wait already gave up
+      if (another_gave_up(status)) return false;
       if (clock64() - t0 > limit) {  // a copy or an arrival was lost; report and leave
-        if (atomicCAS(status, 0, 1) == 0) {
-          status[1] = blockIdx.x;
-          status[2] = where;
-        }
-        return false;
-      }
-    }
-  }
-}
-
-// The same bounded wait for a warp whose wake-up latency sits on the critical path (the issuing warp of the
-// tcgen05 kernel): it spins on the non-blocking test instead of parking.
-__device__ __forceinline__ bool spin_or_flag(uint64_t* bar, uint32_t parity, int32_t* status, int where) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (uint32_t spin = 1;; ++spin) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((spin & 1023u) == 0u) {
-      if (*reinterpret_cast<volatile int32_t*>(status) != 0) return false;
-      if (clock64() - t0 > 4000000000LL) {
-        if (atomicCAS(status, 0, 1) == 0) {
-          status[1] = blockIdx.x;
-          status[2] = where;
-        }
+        report_lost(status, where);
         return false;
       }
     }

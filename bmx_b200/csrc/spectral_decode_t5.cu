@@ -541,8 +541,8 @@ __global__ void __launch_bounds__(S5_THREADS, 1) spectral_decode_t5_kernel(const
           idle = 0;
         } else if ((++idle & 255u) == 0u) {
           if (idle == 256u) t_last = clock64();
-          if (clock64() - t_last > 4000000000LL || *reinterpret_cast<volatile int32_t*>(p.status) != 0) {
-            if (el && atomicCAS(p.status, 0, 1) == 0) p.status[1] = blockIdx.x, p.status[2] = 1;
+          if (clock64() - t_last > 4000000000LL || another_gave_up(p.status)) {
+            if (el) report_lost(p.status, 1);
             ok = false;
           }
         }
@@ -600,8 +600,8 @@ __global__ void __launch_bounds__(S5_THREADS, 1) spectral_decode_t5_kernel(const
               // the buffer still serves the range before the previous one until all its tiles are handed back
               const long long c0 = clock64();
               while (sh->released < first_prev) {
-                if (clock64() - c0 > 4000000000LL || *reinterpret_cast<volatile int32_t*>(p.status) != 0) {
-                  if (atomicCAS(p.status, 0, 1) == 0) p.status[1] = blockIdx.x, p.status[2] = 4;
+                if (clock64() - c0 > 4000000000LL || another_gave_up(p.status)) {
+                  report_lost(p.status, 4);
                   alive = false;
                   break;
                 }
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(S5_THREADS, 1) spectral_decode_t5_kernel(const
           idle = 0;
         } else if ((++idle & 255u) == 0u) {
           if (idle == 256u) t_last = clock64();
-          if (clock64() - t_last > 4000000000LL || *reinterpret_cast<volatile int32_t*>(p.status) != 0) {
-            if (el && atomicCAS(p.status, 0, 1) == 0) p.status[1] = blockIdx.x, p.status[2] = 5;
+          if (clock64() - t_last > 4000000000LL || another_gave_up(p.status)) {
+            if (el) report_lost(p.status, 5);
             ok = false;
           }
         }

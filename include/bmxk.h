@@ -488,7 +488,8 @@ int bmxk_step_ingest(const void* q_src, void* q_dst, int n_q_groups, const void*
 
 
 /* Reads back the status word of the last decode on this workspace (host-synchronising; for
- * tests and diagnostics).  Returns BMXK_ERR_DEVICE if a bounded wait ran out. */
+ * tests and diagnostics).  Returns BMXK_ERR_DEVICE if a bounded wait ran out (1), a window was full (2) or rearranged rotation tables were
+ * too few (3).  The word stays until its owner clears it; after a 1 the waits of later steps on it end early, a 2 or 3 leaves them be. */
 int bmxk_check_workspace_status(const void* workspace, void* stream);
 
 /* Self-test of the bounded device waits (no counterpart in bmx).  Every wait inside the decode kernels (on a bulk
