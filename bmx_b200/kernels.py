@@ -12,6 +12,7 @@ import ctypes
 import functools
 import itertools
 import struct
+import warnings
 
 import torch
 
@@ -461,9 +462,10 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
                         v_tail: torch.Tensor | None, tail_len: torch.Tensor | None, v_lut: torch.Tensor, signs: torch.Tensor, sm_scale: float,
                         status: torch.Tensor, window: int, sinks: int = 0, out: torch.Tensor | None = None, n_split: int | None = None) -> torch.Tensor:
     """k2b_prefill under a sliding window: row i of q (batch, heads, n_q, 128) fp16 stands at position x = q_pos0 + i and sees the
-    keys in (x - window, x] and the first `sinks` up to x.  Pages that no row sees are not read.  rope: rope_fragments() of every page held
-    up to the last row's position (too few are reported in the status word), or None (the tables are read as they are).  status: zeroed
-    device memory (a decode workspace serves).  n_split: shares of a block's page walk, by default what fills the GPU.  A window row that
+    keys in (x - window, x] and the first `sinks` up to x.  Pages that no row sees are not read.  rope: rope_fragments() of every page up
+    to the last row's position, max_pages at most, or None (the tables are read as they are); fewer draw a RuntimeWarning, and if a page
+    behind them is held it is left out and the status word says so (check_status).  status: zeroed device memory (a decode workspace
+    serves).  n_split: shares of a block's page walk, by default what fills the GPU.  A window row that
     some query of a block of 128 // n_q_groups positions sees has to hold finite values."""
     g = pool.geom
     assert q.dim() == 4 and q.shape[2] >= 1
@@ -473,6 +475,10 @@ def k2b_prefill_sliding(pool: K2bPool, q: torch.Tensor, q_pos0: int, basis_f16: 
         assert status.numel() * status.element_size() >= 16 and status.is_contiguous()
         assert basis_f16.dtype is torch.float16 and basis_f16.is_contiguous() and basis_f16.numel() == g.h_kv * HEAD_DIM * g.rank  # read even without pages
         rope_pages = _check_fragments(rope, 0)
+        reach = min(max_pages, max(0, q_pos0 + n_q - 1) // g.page + 1)
+        if 0 < rope_pages < reach:
+            warnings.warn(f"rotation tables rearranged for {rope_pages} pages, the last row's position reaches {reach}: keys behind them are "
+                          "left out if they are held", RuntimeWarning, stacklevel=2)
         out = _check_out(out, q, (torch.float16,))
         if n_split is None:
             pp = max(1, 128 // g.n_q_groups)

@@ -1,0 +1,53 @@
+"""What the steps under a sliding window and over shared prefixes make of their arguments on the host, before any launch: the library call is
+replaced by one that records, so no GPU is needed."""
+
+import contextlib
+import warnings
+
+import pytest
+import torch
+
+from bmx_b200 import kernels as K
+
+D = 128
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The library calls that were made; tensors on the CPU pass for the device's."""
+    made = []
+    K.v_lut_tensor(K.GAUSSIAN_CODEBOOK[2], "cpu")                 # made by the library once, kept from then on
+    monkeypatch.setattr(K, "call", lambda name, *a: made.append((name, a)))
+    monkeypatch.setattr(K, "_on_device_of", lambda *ts: contextlib.nullcontext())
+    monkeypatch.setattr(K, "_stream", lambda: None)
+    monkeypatch.setattr(K, "sm_count", lambda device: 148)
+    return made
+
+
+def _operands(batch=2, h_kv=1, G=4, columns=8, cap=192):
+    g = K.k2b_geom(h_kv, G, 128, 16, 64, h_kv)
+    cos = torch.zeros(128 * columns, D, dtype=torch.float16)
+    win = torch.zeros(batch, h_kv, cap, D, dtype=torch.float16)
+    return dict(pool=K.K2bPool(g, 4, "cpu"), basis=torch.zeros(h_kv * D, 16, dtype=torch.float16), table=torch.zeros(batch, columns, dtype=torch.int32),
+                n_pages=torch.zeros(batch, dtype=torch.int32), cos=cos, win=win, tail=torch.zeros(batch, dtype=torch.int32),
+                lut=K.v_lut_tensor(K.GAUSSIAN_CODEBOOK[2], "cpu"), signs=torch.ones(D), ws=torch.zeros(1 << 16, dtype=torch.uint8))
+
+
+def _prompt(o, rows, pos0, max_pages, fragments, **kw):
+    q = torch.zeros(2, 4, rows, D, dtype=torch.float16)
+    rope = None if fragments is None else torch.zeros(fragments, 8192, dtype=torch.int32)
+    return K.k2b_prefill_sliding(o["pool"], q, pos0, o["basis"], o["table"], o["n_pages"], max_pages, o["cos"], o["cos"], rope, o["win"], o["win"], o["tail"],
+                                 o["lut"], o["signs"], 0.1, o["ws"], 100, 4, **kw)
+
+
+@pytest.mark.parametrize("rows,pos0,max_pages,enough", [(64, 736, 5, 5), (64, 736, 8, 7), (1, 0, 8, 1), (200, 0, 8, 2), (128, 0, 8, 1), (129, 0, 8, 2), (64, 5000, 6, 6)])
+def test_a_prompt_beyond_its_rearranged_tables_draws_a_warning(calls, rows, pos0, max_pages, enough):
+    o = _operands()
+    for n in (enough, enough + 1, None):
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            _prompt(o, rows, pos0, max_pages, n)
+    assert len(calls) == 3 and all(name == "bmxk_k2b_prefill_sliding" for name, _ in calls)
+    if enough > 1:
+        with pytest.warns(RuntimeWarning, match="left out"):
+            _prompt(o, rows, pos0, max_pages, enough - 1)
