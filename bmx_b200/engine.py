@@ -227,8 +227,11 @@ class K2bLayerState:
     def prefill_attend(self, q: torch.Tensor, q_pos0: int, out: torch.Tensor | None = None) -> torch.Tensor | None:
         """Causal attention of q (batch, heads, n_q, 128) fp16 at positions q_pos0 .. over everything held (pages + window),
         page by page, never materialising dense K / V (bmx dequantizes every page first: src/bmx/cache/chunked_attention.py
-        :320-395).  Returns None when this state has no such kernel (64-token pages): the caller takes the dense route."""
+        :320-395).  Returns None when this state has no such kernel (64-token pages): the caller takes the dense route.  Under a
+        sliding window there is no such route (it attends to everything), so that is NotImplementedError."""
         if type(self) is not K2bLayerState or self.geom.layout != 1 or self.geom.n_q_groups not in (1, 2, 4, 8):
+            if self.sliding_window is not None:
+                raise NotImplementedError(f"prompt rows under a sliding window: 1, 2, 4 or 8 query heads per KV head, not {self.geom.n_q_groups}")
             return None
         if self.sliding_window is not None:
             last = max(0, q_pos0 + q.shape[2] - 1) // self.page + 1

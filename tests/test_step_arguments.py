@@ -51,3 +51,15 @@ def test_a_prompt_beyond_its_rearranged_tables_draws_a_warning(calls, rows, pos0
     if enough > 1:
         with pytest.warns(RuntimeWarning, match="left out"):
             _prompt(o, rows, pos0, max_pages, enough - 1)
+
+
+@pytest.mark.parametrize("G", [3, 5, 6, 7])
+def test_prompt_rows_under_a_window_have_no_dense_route(G):
+    """None sends the caller to attention over everything held: a state with a window never answers so."""
+    from bmx_b200.engine import K2bLayerState
+
+    cos = torch.zeros(256, D, dtype=torch.float16)
+    q = torch.zeros(1, G, 5, D, dtype=torch.float16)
+    assert K2bLayerState(K.k2b_geom(1, G), 1, 256, 64, "cpu", cos, cos).prefill_attend(q, 0) is None
+    with pytest.raises(NotImplementedError):
+        K2bLayerState(K.k2b_geom(1, G), 1, 256, 64, "cpu", cos, cos, sliding_window=50, sinks=4).prefill_attend(q, 0)
