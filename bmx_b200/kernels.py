@@ -434,6 +434,8 @@ def _check_out(out: torch.Tensor | None, q: torch.Tensor, dtypes: tuple) -> torc
     if out is None:
         return torch.empty_like(q)
     _require_device_visible(out)
+    if out.is_cuda and out.get_device() != q.get_device():
+        raise RuntimeError(f"tensors of one call lie on different devices: {q.get_device()} and {out.get_device()}")
     assert out.dtype in dtypes and out.is_contiguous() and out.shape == q.shape
     return out
 

@@ -63,3 +63,30 @@ def test_prompt_rows_under_a_window_have_no_dense_route(G):
     assert K2bLayerState(K.k2b_geom(1, G), 1, 256, 64, "cpu", cos, cos).prefill_attend(q, 0) is None
     with pytest.raises(NotImplementedError):
         K2bLayerState(K.k2b_geom(1, G), 1, 256, 64, "cpu", cos, cos, sliding_window=50, sinks=4).prefill_attend(q, 0)
+
+
+class _On:
+    """Stands for a tensor of a device (None: pinned host memory)."""
+
+    def __init__(self, device, like):
+        self.device_index, self.is_cuda = device, device is not None
+        self.dtype, self.shape = like.dtype, like.shape
+
+    def is_contiguous(self):
+        return True
+
+    def is_pinned(self):
+        return True
+
+    def get_device(self):
+        return -1 if self.device_index is None else self.device_index
+
+
+def test_an_output_on_another_device_is_refused():
+    like = torch.zeros(2, 4, D, dtype=torch.float16)
+    q = _On(1, like)
+    for where in (1, None):
+        out = _On(where, like)
+        assert K._check_out(out, q, (torch.float16,)) is out
+    with pytest.raises(RuntimeError, match="different devices: 1 and 0"):
+        K._check_out(_On(0, like), q, (torch.float16,))
