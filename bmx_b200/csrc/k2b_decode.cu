@@ -1018,6 +1018,10 @@ static int check_step(const bmxk_k2b_geom* g, const void* q, const void* pages, 
   BMXK_REQUIRE(out_dtype == BMXK_DTYPE_F16 || out_dtype == BMXK_DTYPE_F32, "bmxk_k2b_decode: out_dtype=%d", out_dtype);
   BMXK_REQUIRE(workspace_bytes >= bmxk_k2b_decode_workspace_bytes(g, batch, max_pages), "bmxk_k2b_decode: workspace too small");
   BMXK_REQUIRE(((uintptr_t)pages & 15) == 0 && ((uintptr_t)coefs & 15) == 0, "bmxk_k2b_decode: pools must be 16-byte aligned");
+  // read by words, by 16 bytes where the operand is copied to shared memory or to registers whole
+  BMXK_REQUIRE(max_pages == 0 || ((((uintptr_t)rope_cos | (uintptr_t)rope_sin) & 3) == 0 && ((uintptr_t)basis_f16 & (g->layout == 1 ? 15 : 3)) == 0),
+               "bmxk_k2b_decode: rotation tables must be 4-byte aligned, the basis %d-byte aligned", g->layout == 1 ? 16 : 4);
+  BMXK_REQUIRE(tail_cap == 0 || (((uintptr_t)k_tail | (uintptr_t)v_tail) & 15) == 0, "bmxk_k2b_decode: windows must be 16-byte aligned");
   return BMXK_OK;
 }
 

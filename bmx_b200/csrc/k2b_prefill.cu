@@ -503,6 +503,7 @@ static int prefill_impl(const bmxk_k2b_geom* g, const void* q, int n_q, int64_t 
   BMXK_REQUIRE(tail_cap == 0 || (k_tail && v_tail && tail_len), "bmxk_k2b_prefill: null window");
   BMXK_REQUIRE(((uintptr_t)pages & 15) == 0 && ((uintptr_t)coefs & 15) == 0 && ((uintptr_t)basis_f16 & 15) == 0 &&
                    ((uintptr_t)rope_cos & 15) == 0 && ((uintptr_t)rope_sin & 15) == 0 && ((uintptr_t)q & 3) == 0 && ((uintptr_t)out & 3) == 0 &&
+                   ((uintptr_t)status & 3) == 0 &&
                    (tail_cap == 0 || ((((uintptr_t)k_tail | (uintptr_t)v_tail) & 15) == 0)),
                "bmxk_k2b_prefill: misaligned buffer");
   PrefillParams prm;

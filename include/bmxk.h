@@ -137,7 +137,8 @@ size_t bmxk_k2b_decode_workspace_bytes(const bmxk_k2b_geom* g, int batch, int ma
  * phases: 3 runs the whole step; 1 launches only the page-streaming kernel and 2 only the merge
  * kernel (same arguments), so that a caller can time them apart.
  * workspace: device memory of bmxk_k2b_decode_workspace_bytes(), zero-filled once by the caller
- * (its first 16 bytes are a status word that a kernel sets only if a bounded wait ran out). */
+ * (its first 16 bytes are a status word, see bmxk_check_workspace_status).
+ * Pools, windows and (layout 1) the basis begin on 16 bytes, rotation tables on 4; q on any fp16. */
 int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs,
                     const void* basis_f16, const int32_t* page_table, int table_stride, const int32_t* n_pages,
                     int batch, int max_pages, const void* rope_cos, const void* rope_sin, int64_t pos_offset,

@@ -2,11 +2,13 @@
 replaced by one that records, so no GPU is needed."""
 
 import contextlib
+import ctypes
 import warnings
 
 import pytest
 import torch
 
+from bmx_b200 import _lib
 from bmx_b200 import kernels as K
 
 D = 128
@@ -90,3 +92,38 @@ def test_an_output_on_another_device_is_refused():
         assert K._check_out(out, q, (torch.float16,)) is out
     with pytest.raises(RuntimeError, match="different devices: 1 and 0"):
         K._check_out(_On(0, like), q, (torch.float16,))
+
+
+def _step(which, layout=1, page=128, rank=16, G=4, a=4096, tail_cap=192, **at):
+    """A step on made-up addresses that nothing reads; `at` moves operands.  (status, message)."""
+    lib, g = _lib.lib(), _lib.K2bGeom(2, G, page, rank, 64, 2, 3, 2, layout)
+    p = {k: a + at.get(k, 0) for k in ("q", "basis", "cos", "sin", "k", "v", "out", "ws")}
+    head = (ctypes.byref(g), p["q"], a, a, p["basis"], a, 3, a)
+    lut, big = (ctypes.c_uint32 * 4)(), 1 << 40
+    if which == "plain":
+        rc = lib.bmxk_k2b_decode(*head, 2, 3, p["cos"], p["sin"], 0, p["k"], p["v"], a, tail_cap, lut, a, 0.1, p["ws"], big, p["out"], 0, None, 3, None)
+    elif which == "sliding":
+        rc = lib.bmxk_k2b_decode_sliding(*head, 2, 3, p["cos"], p["sin"], p["k"], p["v"], a, tail_cap, lut, a, 0.1, 100, 4, p["ws"], big, p["out"], 0, None)
+    elif which == "shared":
+        rc = lib.bmxk_k2b_decode_shared(*head, 2, 3, 2, a, a, a, 0, 0, 1, p["cos"], p["sin"], None, 0, p["k"], p["v"], a, tail_cap, lut, a, 0.1, p["ws"], big,
+                                        p["out"], 0, None)
+    else:
+        rc = lib.bmxk_k2b_prefill_sliding(ctypes.byref(g), p["q"], 8, 0, a, a, p["basis"], a, 3, a, 1, p["cos"], p["sin"], None, 0, p["k"], p["v"], a, tail_cap,
+                                          lut, a, 0.1, 100, 4, p["ws"], p["out"], 1, None, 0, None)
+    return rc, lib.bmxk_last_error()
+
+
+@pytest.mark.parametrize("which", ["plain", "sliding", "shared", "prompt"])
+@pytest.mark.parametrize("operand,by", [("cos", 2), ("sin", 2), ("basis", 8), ("basis", 2), ("k", 8), ("v", 2)])
+def test_operands_that_are_read_by_words_are_aligned(which, operand, by):
+    """Whatever a kernel reads by words or 16 bytes at a time is refused elsewhere, not met on the device."""
+    rc, message = _step(which, **{operand: by})
+    assert rc == _lib.BMXK_ERR_INVALID and b"align" in message, message
+
+
+def test_64_token_pages_and_status_words_are_aligned_too():
+    for operand, by in (("cos", 2), ("basis", 2), ("k", 8)):
+        rc, message = _step("plain", layout=0, page=64, **{operand: by})
+        assert rc == _lib.BMXK_ERR_INVALID and b"align" in message, message
+    rc, message = _step("prompt", ws=1)
+    assert rc == _lib.BMXK_ERR_INVALID and b"align" in message, message
