@@ -926,11 +926,21 @@ static size_t group_merge_smem(int G, int tail_cap) {
   return ((size_t)gq * ((tail_cap + 3) & ~3) + 8 * gq * HEAD_DIM + 4 * HEAD_DIM + 24 + 4) * sizeof(float);
 }
 
+static size_t plain_merge_smem(int tail_cap) { return ((size_t)((tail_cap + 3) & ~3) + (1 + 16 + 1) * HEAD_DIM + 32 + 4) * sizeof(float); }
+
+// Whether the merge kernel's shared memory holds a window's scores.
+static int check_merge(int G, int tail_cap, int walk) {
+  BMXK_REQUIRE(walk == WALK_ALL ? plain_merge_smem(tail_cap) <= 48 * 1024 : group_merge_smem(G, tail_cap) <= GROUP_MERGE_SMEM,
+               "decode: tail_cap=%d too large for the merge kernel", tail_cap);
+  return BMXK_OK;
+}
+
 int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int walk) {
   const int G = mp.g.n_q_groups, gq = G <= 4 ? 4 : 8;
+  const int bad = check_merge(G, mp.tail_cap, walk);
+  if (bad) return bad;
   if (walk != WALK_ALL) {
     size_t gsmem = group_merge_smem(G, mp.tail_cap);
-    BMXK_REQUIRE(gsmem <= GROUP_MERGE_SMEM, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
     // While the page-streaming kernel drains, the blocks would pile up three to an SM on the SMs that are free already; a block that asks for
     // more shared memory keeps them apart as long as the grid is small enough to spread (256 pairs: 63 -> 60 us a step; 128 pairs 52 -> 47).
     // The blocks of eight query heads are two to an SM by their registers; one to an SM starts too late (126 pairs: 37 -> 41 us).
@@ -940,10 +950,8 @@ int launch_merge(const K2bMergeParams& mp, cudaStream_t s, bool after_main, int 
     if (walk == WALK_OWN) return gq == 4 ? launch_merge_group<WALK_OWN, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_OWN, 8>(mp, gsmem, s, after_main);
     return gq == 4 ? launch_merge_group<WALK_SLIDING, 4>(mp, gsmem, s, after_main) : launch_merge_group<WALK_SLIDING, 8>(mp, gsmem, s, after_main);
   }
-  const size_t msmem = ((size_t)((mp.tail_cap + 3) & ~3) + (1 + 16 + 1) * HEAD_DIM + 32 + 4) * sizeof(float);
-  BMXK_REQUIRE(msmem <= 48 * 1024, "decode: tail_cap=%d too large for the merge kernel", mp.tail_cap);
   const unsigned grid = (unsigned)(mp.batch * mp.g.h_kv * G);
-  return launch_merge_kernel(k2b_merge_kernel, mp, grid, msmem, s, after_main);
+  return launch_merge_kernel(k2b_merge_kernel, mp, grid, plain_merge_smem(mp.tail_cap), s, after_main);
 }
 
 static size_t decode_stage_bytes(const bmxk_k2b_geom* g) {
@@ -1044,6 +1052,8 @@ static int decode_step(const bmxk_k2b_geom* g, const void* q, const void* pages,
   const int bad = check_step(g, q, pages, coefs, basis_f16, page_table, n_pages, batch, max_pages, rope_cos, rope_sin, k_tail, v_tail, tail_len,
                              tail_cap, v_lut, signs, workspace, workspace_bytes, out, out_dtype, partial_out, phases);
   if (bad) return bad;
+  const int wide = (phases & 2) ? check_merge(g->n_q_groups, tail_cap, walk) : BMXK_OK;
+  if (wide) return wide;
   cudaStream_t s = (cudaStream_t)stream;
 
   int32_t* status = reinterpret_cast<int32_t*>(workspace);
@@ -1165,7 +1175,8 @@ int bmxk_k2b_decode_shared(const bmxk_k2b_geom* g, const void* q, const void* pa
   if (off) return off;
   const int large = check_decode_t5(g->rank, g->group, batch, WALK_OWN);
   if (large) return large;
-  BMXK_REQUIRE(group_merge_smem(g->n_q_groups, tail_cap) <= GROUP_MERGE_SMEM, "bmxk_k2b_decode_shared: tail_cap=%d too large for the merge kernel", tail_cap);
+  const int wide = check_merge(g->n_q_groups, tail_cap, WALK_OWN);
+  if (wide) return wide;
   const bool prefixes = n_groups > 0 && max_members > 0 && max_pages > 0;
   float* part = reinterpret_cast<float*>((uint8_t*)workspace + (bmxk_k2b_decode_workspace_bytes(g, batch, 0) + 255) / 256 * 256);
   if (prefixes) {

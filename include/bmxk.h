@@ -152,7 +152,8 @@ int bmxk_k2b_decode(const bmxk_k2b_geom* g, const void* q, const void* pages, co
  * < sinks.  Arguments as in bmxk_k2b_decode (no pos_offset, no partial states); layout 1 only.  Pages without a visible token are not
  * read and their page-table entries may be anything: a caller frees them.  No per-step argument.  A sequence that holds nothing gives 0.
  * q, basis, windows, workspace (bmxk_k2b_decode_workspace_bytes) and out are 16-byte aligned; calls that may run at the same time need
- * workspaces of their own.
+ * workspaces of their own.  Refused before anything is launched: tail_cap above what the merge's shared memory holds scores for (11000 always
+ * fits at up to four query heads per KV head, 5000 above).
  * (bmx's cache attends to everything it holds: src/bmx/cache/chunked_attention.py:398-530; a model's sliding layers have no path there.) */
 int bmxk_k2b_decode_sliding(const bmxk_k2b_geom* g, const void* q, const void* pages, const void* coefs, const void* basis_f16,
                             const int32_t* page_table, int table_stride, const int32_t* n_pages, int batch, int max_pages, const void* rope_cos,

@@ -127,3 +127,9 @@ def test_64_token_pages_and_status_words_are_aligned_too():
         assert rc == _lib.BMXK_ERR_INVALID and b"align" in message, message
     rc, message = _step("prompt", ws=1)
     assert rc == _lib.BMXK_ERR_INVALID and b"align" in message, message
+
+
+@pytest.mark.parametrize("which,G,tail_cap", [("sliding", 8, 9000), ("sliding", 5, 6000), ("sliding", 4, 12000), ("shared", 8, 9000), ("plain", 4, 12000)])
+def test_a_window_that_the_merge_cannot_hold_is_refused_before_the_first_launch(which, G, tail_cap):
+    rc, message = _step(which, G=G, tail_cap=tail_cap)
+    assert rc == _lib.BMXK_ERR_INVALID and b"tail_cap=%d" % tail_cap in message, message
