@@ -244,6 +244,9 @@ class PagedK2bLayer:
         moved, holes = self.alloc.compact()
         now = dict(zip(moved, holes))
         K.copy_slots([old.pages, old.coefs], [pool.pages, pool.coefs], live, [now.get(s, s) for s in live])
+        for t in (old.pages, old.coefs):  # their memory may belong to another stream, which must not hand it out while this one copies
+            if t.is_cuda:
+                t.record_stream(torch.cuda.current_stream(self.device))
         self.pool = pool
         if n_slots > self.alloc.n_slots:
             self.alloc.grow(n_slots - self.alloc.n_slots)

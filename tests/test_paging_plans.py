@@ -130,3 +130,25 @@ def test_steps_get_what_the_sequences_hold_whatever_happened_in_between(monkeypa
                 seqs = rng.sample(live, rng.randint(1, len(live)))
             kinds.add(b.step(seqs))
     assert kinds == ({"k2b_decode", "k2b_decode_shared"} if not kw else {"k2b_decode_sliding"})
+
+
+def test_a_pool_that_is_replaced_stays_until_the_copying_stream_is_through(monkeypatch):
+    """A pool belongs to the stream it was made on; resized on another one, it is not free before that one has copied it."""
+
+    class Held:
+        is_cuda = True
+
+        def __init__(self):
+            self.streams = []
+
+        def record_stream(self, stream):
+            self.streams.append(stream)
+
+    b = Steps(monkeypatch, slots=10)
+    b.start("a", 500)
+    old = b.layer.pool
+    old.pages, old.coefs = Held(), Held()
+    b.stream = types.SimpleNamespace(cuda_stream=9)
+    b.layer.resize(20)
+    assert b.layer.pool is not old and old.pages.streams == [b.stream] and old.coefs.streams == [b.stream]
+    b.step(["a"])
