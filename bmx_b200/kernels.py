@@ -566,6 +566,8 @@ def k2b_decode_shared(pool: K2bPool, q: torch.Tensor, basis_f16: torch.Tensor, p
         batch, stride, tail_cap = _check_step(pool, q, page_table, n_pages, max_pages, basis_f16, rope_cos, rope_sin, k_tail, v_tail, tail_len, v_lut, signs)
         assert groups.max_prefix <= max_pages, f"a prefix of {groups.max_prefix} pages, {max_pages} held at most"
         rope_pages = _check_fragments(rope, groups.max_prefix)
+        assert rope is not None or groups.max_prefix == 0 or 128 * groups.max_prefix <= min(rope_cos.shape[0], rope_sin.shape[0]), \
+            f"rotation tables end before the {groups.max_prefix} pages of a prefix"
         own = max_pages - groups.min_prefix
         out = _check_out(out, q, (torch.float16, torch.float32))
         call("bmxk_k2b_decode_shared", ctypes.byref(g), _addr(q), _addr(pool.pages), _addr(pool.coefs), _addr(basis_f16), _addr(page_table),

@@ -133,3 +133,22 @@ def test_64_token_pages_and_status_words_are_aligned_too():
 def test_a_window_that_the_merge_cannot_hold_is_refused_before_the_first_launch(which, G, tail_cap):
     rc, message = _step(which, G=G, tail_cap=tail_cap)
     assert rc == _lib.BMXK_ERR_INVALID and b"tail_cap=%d" % tail_cap in message, message
+
+
+@pytest.mark.parametrize("rows,fine", [(1024, True), (1023, False), (900, False)])
+def test_rotation_tables_that_end_inside_a_prefix_are_refused(calls, rows, fine):
+    """The prefix kernel reads the row of every position of its pages where the tables are not rearranged."""
+    o = _operands()
+    groups = K.PrefixGroups(o["pool"].geom, 2, [[0, 1]], [8], "cpu", n_split=1)
+
+    def step(cos, sin):
+        K.k2b_decode_shared(o["pool"], torch.zeros(2, 4, D, dtype=torch.float16), o["basis"], o["table"], o["n_pages"], 8, groups, cos, sin, None, o["win"],
+                            o["win"], o["tail"], o["lut"], o["signs"], 0.1, o["ws"])
+
+    for cos, sin in ((o["cos"][:rows], o["cos"]), (o["cos"], o["cos"][:rows])):
+        if fine:
+            step(cos, sin)
+        else:
+            with pytest.raises(AssertionError, match="8 pages"):
+                step(cos, sin)
+    assert len(calls) == 2 * fine
