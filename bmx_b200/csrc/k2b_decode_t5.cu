@@ -28,6 +28,11 @@
 // which it reads with independent loads (an mbarrier test costs ~70 cycles and tests do not overlap), and
 // per-tile facts it would have to derive (basis buffer, first tile of a range) are left for it in shared
 // memory by the rotation warps.  The two parities end as two partial records per (CTA, range).
+//
+// Rounded to fewer than 32 bits: K_low (fp16 accumulators over rank / 16 products of 16), the key after its residual and the products of its
+// rotation (half2), because the key warps' instructions bound the kernel and 32 bits would double them; the rotated query, weight x norm and the value
+// levels, which are fp16 operands of the contractions.  Running maxima, sums and accumulators are in 32 bits, and so are the scores and
+// weights of the fp16 window in the merge kernels.
 #include "decode_common.cuh"
 #include "tc5.cuh"
 

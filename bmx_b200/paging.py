@@ -150,13 +150,17 @@ class PagedK2bLayer:
     `fork` makes sequences that share all committed pages of another one; a decode step that meets several sequences with a common
     prefix reads it once for all of them.  With sliding_window, a token sees the last sliding_window tokens and the first `sinks`; pages
     that fall between the two are freed as sequences grow.  `compact` and `resize` close the holes that finished sequences leave.
+    A sequence's length is limited by max_pages_per_seq pages, freed ones among them (its page table keeps their places), and by the
+    rotation tables.
     """
 
     # 128-token tiles per SM that attending shared prefixes once has to save over streaming them for every sequence; its launch and the set-up of
-    # its blocks cost the time of about one.  Measured at 8 KV heads and up to 3 pages behind the prefixes, shared against streamed: 4 query
-    # heads per KV head, 4 sequences x 2 pages (0.3 tiles per SM saved) 15 against 13 us, 4 x 4 (0.7) 15 against 17, 8 x 4 (1.5) 15 against 19, 32 x
-    # 256 49 against 402; 1 query head, 4 x 4 (0.7) 15 against 16, 2 x 16 (0.9) 16 against 14, 3 x 16 (1.7) 16 against 15, 8 x 8 (3.0) 15 against 18; 8
-    # query heads, 4 x 1 (0.2) 16 against 18, 2 x 8 (0.4) 17 against 20.
+    # its blocks cost the time of about one.  Measured at 8 KV heads and up to 3 pages behind the prefixes, steps in a replayed graph, shared
+    # against streamed, in us.  Shared by this rule: 4 query heads per KV head, 2 sequences x 20 pages (1.1 tiles per SM saved) 15.7 / 15.7,
+    # 8 x 4 (1.5) 16.7 / 18.3, 32 x 4 (6.7) 22.2 / 42.5, 32 x 256 49 / 402; 1 query head, 3 x 16 (1.7) 15.5 / 14.9, 6 x 8 (2.2) 15.6 / 17.1, 8 x 8
+    # (3.0) 17.0 / 18.1.  Streamed: 1 query head, 4 x 4 (0.6) 14.9 / 12.5, 2 x 16 (0.9) 15.3 / 13.9; 4 query heads, 4 x 4 (0.6) 15.0 / 16.0, 3 x 8
+    # (0.9) 15.1 / 16.6; 8 query heads, 4 x 1 (0.2) 15.9 / 18.1, 2 x 8 (0.4) 15.9 / 19.4.  The border lies higher with one query head and lower with
+    # eight; one number for all of them is off by at most 0.6 us above it and 3.5 us below.
     SHARED_MIN_TILES = 1
 
     def __init__(self, geom, n_slots: int, max_seqs: int, recent_window: int, device, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
